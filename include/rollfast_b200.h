@@ -303,6 +303,130 @@ rf_status rf_flags_signal(uint32_t* const* flags, int32_t n, uint32_t value, voi
 rf_status rf_flags_wait(const uint32_t* flags, int32_t n, int32_t skip, uint32_t target, double timeout_s,
                         void* stream);
 
+/* ------------------------------------------------------------------------
+ * The training step around the optimizer: activations saved in 8 bits, the
+ * weight gradient and a SwiGLU that read them, and the norms around a block.
+ * No reference counterpart (there, XLA differentiates the model); each
+ * operator is a forward / backward pair, as a custom derivative rule binds
+ * them.
+ * ------------------------------------------------------------------------ */
+
+/* An activation in 8 bits.  A row of features is cut into blocks of 32: 32
+ * codes (int8, or e4m3) and one byte s, value = code * 2^(s - 127), with s
+ * the smallest in [1, top] for which max|x| <= 127 * 2^(s - 127) (448 for
+ * e4m3; top 248, 246: larger magnitudes saturate there).  s = 255 marks a
+ * block that held an infinity or a NaN; all of it reads as NaN.
+ *   codes   [rows][ld] bytes, ld = features rounded up to 16
+ *   scales  [ceil(features / 128)][scale_rows][4] bytes s, one for each block
+ *           of a panel of 128 features; scale_rows = rows rounded up to 64
+ * Both 16-byte aligned.  At most 2^31 - 1 rows and 2^26 features. */
+typedef enum rf_format8 { RF_INT8 = 0, RF_E4M3 = 1 } rf_format8;
+typedef struct rf_saved_activation {
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t rows, features;
+  int64_t ld, scale_rows;
+  int32_t format;  /* rf_format8 */
+} rf_saved_activation;
+
+/* Row strides (ld*) below are in elements; a row's elements are contiguous. */
+
+/* x [rows][features] -> codes and steps, to nearest even, or stochastically:
+ * a value between two grid points goes to the upper one with the probability
+ * of its distance from the lower (mean = value, so gradients that are linear
+ * in it stay unbiased), by 16 bits per element of the SplitMix64 sequence of
+ * `seed`, in element order as in rf_apply_updates. */
+rf_status rf_save_activation(const void* x, int64_t ldx, int32_t dtype, const rf_saved_activation* out,
+                             int32_t stochastic, uint64_t seed, void* stream);
+/* The values, rounded to `dtype` (exact in float32 and bfloat16 but for
+ * subnormals; float16 saturates at 65504). */
+rf_status rf_load_activation(const rf_saved_activation* saved, void* out, int64_t ldo, int32_t dtype, void* stream);
+
+/* h = silu(gate) * up, and (both or neither) the inputs saved in 8 bits. */
+rf_status rf_swiglu_forward(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, void* h, int64_t ld_h,
+                            int32_t dtype, int64_t rows, int64_t features, const rf_saved_activation* saved_gate,
+                            const rf_saved_activation* saved_up, void* stream);
+/* The gradients at the saved inputs, and (saved_h not NULL) h formed again
+ * from them and saved, for the weight gradient of the product that reads it. */
+rf_status rf_swiglu_backward(const void* grad_h, int64_t ld_grad, const rf_saved_activation* saved_gate,
+                             const rf_saved_activation* saved_up, void* grad_gate, int64_t ld_gate, void* grad_up,
+                             int64_t ld_up, int32_t dtype, const rf_saved_activation* saved_h, void* stream);
+
+/* Weight gradient of y = x W from the saved x: with X [rows][features] the
+ * saved values and G [rows][n_out] = grad_out,
+ *   layout RF_IN_OUT: out[i][o] = initial[i][o] + sum_t X[t][i] G[t][o]
+ *   layout RF_OUT_IN: out[o][i], the transpose
+ * in float32, rounded once to out_dtype.  `initial` (out's shape, dtype and
+ * stride) may be NULL, or out itself to accumulate in place.  X enters the
+ * tensor cores exactly; float16 and float32 gradients enter as two and three
+ * bfloat16 terms that add up to them exactly.  rows = 0 writes `initial` or
+ * zeros.  The result does not depend on anything but the operands and their
+ * shapes (no atomics). */
+typedef enum rf_weight_layout { RF_IN_OUT = 0, RF_OUT_IN = 1 } rf_weight_layout;
+rf_status rf_weight_gradient_workspace_size(int64_t rows, int64_t features, int64_t n_out, const void* grad_out,
+                                            int64_t ld_grad, int32_t grad_dtype, size_t* bytes);
+rf_status rf_weight_gradient(const rf_saved_activation* saved, const void* grad_out, int64_t ld_grad,
+                             int32_t grad_dtype, int64_t n_out, int32_t layout, const void* initial, void* out,
+                             int64_t ld_out, int32_t out_dtype, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/* The norms around a block, with its gate, residual scale and residual
+ * addition.  For a residual stream x and a block's output b, both
+ * [rows][features]:
+ *   x' = x + scale * act(gate) * N_post(b)        (N_post(b) = b without post_norm)
+ *   y  = N_pre(x')                                (the next block's input)
+ * N normalises a row by its root mean square (RF_RMS_NORM) or by mean and
+ * variance (RF_LAYER_NORM), eps inside the root, then weight and bias where
+ * given.  All in float32, each output rounded once (y comes from the
+ * unrounded x'). */
+typedef enum rf_norm_kind { RF_RMS_NORM = 0, RF_LAYER_NORM = 1 } rf_norm_kind;
+typedef enum rf_gate_act { RF_GATE_IDENTITY = 0, RF_GATE_SIGMOID = 1, RF_GATE_TANH = 2 } rf_gate_act;
+typedef struct rf_norm_param {
+  const void* value;  /* NULL: absent */
+  void* grad;         /* backward: its gradient, same shape and dtype; NULL: not wanted */
+  int32_t dtype;
+} rf_norm_param;
+typedef struct rf_block_norm {
+  int64_t rows, features;     /* at most 2^31 - 1 rows, 16384 features */
+  int32_t kind;               /* rf_norm_kind */
+  int32_t post_norm;
+  float eps;
+  float scale;                /* the residual scale when residual_scale.value is NULL */
+  rf_norm_param pre_weight, pre_bias, post_weight, post_bias;  /* [features]; post_* need post_norm */
+  rf_norm_param residual_scale;  /* [features], or one element */
+  int32_t scale_per_channel;
+  /* One row of gates for each gate_rows rows: [rows / gate_rows][features],
+   * or [rows / gate_rows] without gate_per_channel. */
+  rf_norm_param gate;
+  int64_t gate_rows;
+  int32_t gate_per_channel;
+  int32_t gate_act;           /* rf_gate_act */
+} rf_block_norm;
+/* A row-strided array of a float type, or a saved activation. */
+typedef struct rf_rows {
+  const void* data;                   /* NULL with saved */
+  int64_t ld;
+  int32_t dtype;
+  const rf_saved_activation* saved;   /* backward inputs only */
+} rf_rows;
+
+/* branch.data NULL: y = N_pre(x) alone (x_out unused).  y.data NULL: x' alone.
+ * saved_* (each may be NULL) receive x', b and y in 8 bits, exactly as
+ * rf_save_activation of the stored arrays would. */
+rf_status rf_block_norm_forward(const rf_block_norm* p, const rf_rows* x, const rf_rows* branch, const rf_rows* x_out,
+                                const rf_rows* y, const rf_saved_activation* saved_x,
+                                const rf_saved_activation* saved_branch, const rf_saved_activation* saved_y,
+                                void* stream);
+/* Gradients at x' and b (given as arrays or saved activations), from those of
+ * x' (grad_x, may be absent) and y (grad_y, may be absent):
+ *   e = grad_x + N_pre'(grad_y);  out_x = e;  out_branch = N_post'(scale * act(gate) * e)
+ * and the sums over rows for every parameter with a grad pointer.  Sums are
+ * formed in a fixed order (no atomics). */
+rf_status rf_block_norm_workspace_size(const rf_block_norm* p, size_t* bytes);
+rf_status rf_block_norm_backward(const rf_block_norm* p, const rf_rows* grad_x, const rf_rows* grad_y,
+                                 const rf_rows* x, const rf_rows* branch, const rf_rows* out_x,
+                                 const rf_rows* out_branch, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Diagnostics. */
 const char* rf_last_error(void);
 rf_status rf_version(int32_t* major, int32_t* minor, int32_t* patch);

@@ -23,6 +23,12 @@ RF_PRECOND_FROBENIUS, RF_PRECOND_SPECTRAL, RF_PRECOND_AOL, RF_PRECOND_SCHATTEN =
 PRECONDITIONING_CODES = {"frobenius": RF_PRECOND_FROBENIUS, "spectral": RF_PRECOND_SPECTRAL,
                          "aol": RF_PRECOND_AOL, "schatten": RF_PRECOND_SCHATTEN}
 
+RF_INT8, RF_E4M3 = 0, 1
+FORMAT8_CODES = {"int8": RF_INT8, "e4m3": RF_E4M3}
+RF_IN_OUT, RF_OUT_IN = 0, 1
+RF_RMS_NORM, RF_LAYER_NORM = 0, 1
+RF_GATE_IDENTITY, RF_GATE_SIGMOID, RF_GATE_TANH = 0, 1, 2
+
 PRECISIONS = {"f16": RF_NS_F16, "fp16": RF_NS_F16, "float16": RF_NS_F16,
               "bf16": RF_NS_BF16, "bfloat16": RF_NS_BF16,
               "f32": RF_NS_F32, "fp32": RF_NS_F32, "float32": RF_NS_F32}
@@ -52,6 +58,15 @@ EXPORTED = (
     "rf_peer_copy",
     "rf_flags_signal",
     "rf_flags_wait",
+    "rf_save_activation",
+    "rf_load_activation",
+    "rf_swiglu_forward",
+    "rf_swiglu_backward",
+    "rf_weight_gradient_workspace_size",
+    "rf_weight_gradient",
+    "rf_block_norm_forward",
+    "rf_block_norm_workspace_size",
+    "rf_block_norm_backward",
 )
 
 
@@ -172,6 +187,56 @@ class RfAdamParams(ctypes.Structure):
     ]
 
 
+class RfSavedActivation(ctypes.Structure):
+    _fields_ = [
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("features", ctypes.c_int64),
+        ("ld", ctypes.c_int64),
+        ("scale_rows", ctypes.c_int64),
+        ("format", ctypes.c_int32),
+    ]
+
+
+class RfNormParam(ctypes.Structure):
+    _fields_ = [
+        ("value", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class RfBlockNorm(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("features", ctypes.c_int64),
+        ("kind", ctypes.c_int32),
+        ("post_norm", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("scale", ctypes.c_float),
+        ("pre_weight", RfNormParam),
+        ("pre_bias", RfNormParam),
+        ("post_weight", RfNormParam),
+        ("post_bias", RfNormParam),
+        ("residual_scale", RfNormParam),
+        ("scale_per_channel", ctypes.c_int32),
+        ("gate", RfNormParam),
+        ("gate_rows", ctypes.c_int64),
+        ("gate_per_channel", ctypes.c_int32),
+        ("gate_act", ctypes.c_int32),
+    ]
+
+
+class RfRows(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("ld", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("saved", ctypes.POINTER(RfSavedActivation)),
+    ]
+
+
 class RollfastError(RuntimeError):
     """A non-OK rf_status from the native library."""
 
@@ -226,6 +291,16 @@ def load(path: str | None = None):
         lib.rf_peer_copy.argtypes = [vp, vp, sz, vp]
         lib.rf_flags_signal.argtypes = [ctypes.POINTER(vp), i32, ctypes.c_uint32, vp]
         lib.rf_flags_wait.argtypes = [vp, i32, i32, ctypes.c_uint32, ctypes.c_double, vp]
+        sav, rows, norm = (ctypes.POINTER(RfSavedActivation), ctypes.POINTER(RfRows), ctypes.POINTER(RfBlockNorm))
+        lib.rf_save_activation.argtypes = [vp, i64, i32, sav, i32, ctypes.c_uint64, vp]
+        lib.rf_load_activation.argtypes = [sav, vp, i64, i32, vp]
+        lib.rf_swiglu_forward.argtypes = [vp, i64, vp, i64, vp, i64, i32, i64, i64, sav, sav, vp]
+        lib.rf_swiglu_backward.argtypes = [vp, i64, sav, sav, vp, i64, vp, i64, i32, sav, vp]
+        lib.rf_weight_gradient_workspace_size.argtypes = [i64, i64, i64, vp, i64, i32, ctypes.POINTER(sz)]
+        lib.rf_weight_gradient.argtypes = [sav, vp, i64, i32, i64, i32, vp, vp, i64, i32, vp, sz, vp]
+        lib.rf_block_norm_forward.argtypes = [norm, rows, rows, rows, rows, sav, sav, sav, vp]
+        lib.rf_block_norm_workspace_size.argtypes = [norm, ctypes.POINTER(sz)]
+        lib.rf_block_norm_backward.argtypes = [norm, rows, rows, rows, rows, rows, rows, vp, sz, vp]
         for name in EXPORTED:
             f = getattr(lib, name)
             if name not in ("rf_last_error", "rf_kernel_launch_count"):

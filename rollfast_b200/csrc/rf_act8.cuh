@@ -1,0 +1,250 @@
+// The 8-bit form of a saved activation, and 8-element row access for the
+// kernels that read or write one.
+//
+// A row of features is cut into blocks of 32.  A block holds 32 codes (int8
+// in two's complement, or e4m3) and one byte s: value = code * 2^(s - 127).
+// s is the smallest in [1, top] with max|x| <= 127 * 2^(s - 127) (448 for
+// e4m3), so nothing saturates below the largest step; top (248, 246) is the
+// largest at which every code is finite in float32 and bfloat16, and larger
+// magnitudes saturate there.  s = 255: the block held an infinity or a NaN,
+// and every value of it reads as NaN.  Powers of two make each value exact in
+// bfloat16 (8 significant bits at most), so a tensor-core product over these
+// values has no rounding of its operand.
+//
+// Codes: [rows][ld] bytes, ld = features rounded up to 16, zeros behind the
+// last feature.  Steps: [panels of 128 features][scale_rows][4], scale_rows =
+// rows rounded up to 64, so that the steps of a 64 x 128 tile are 256
+// contiguous bytes; blocks behind the last feature hold 1.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "rf_common.cuh"
+
+namespace rf {
+
+constexpr int kBlock8 = 32;       // features that share a step
+constexpr int kPanel8 = 128;      // features per panel of steps
+constexpr uint32_t kNanStep = 255u;
+constexpr int64_t kMaxFeatures = int64_t(1) << 26;  // keeps column tiles inside a grid's 65535 in y
+
+// A device view of a row-strided array of one of the float types.
+struct RowView {
+  const void* p;
+  int64_t ld;     // elements between rows
+  int32_t dt;     // rf_dtype
+  int32_t vec;    // rows start on 16-byte boundaries
+};
+struct RowOut {
+  void* p;
+  int64_t ld;
+  int32_t dt;
+  int32_t vec;
+};
+struct Saved8 {
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t ld;
+  int64_t scale_rows;
+  int32_t format;
+};
+
+inline bool rows_vectorised(const void* p, int64_t ld, int dt) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * int64_t(dtype_size(dt))) % 16 == 0;
+}
+inline RowView row_view(const void* p, int64_t ld, int dt) { return RowView{p, ld, dt, rows_vectorised(p, ld, dt)}; }
+inline RowOut row_out(void* p, int64_t ld, int dt) { return RowOut{p, ld, dt, rows_vectorised(p, ld, dt)}; }
+inline Saved8 saved8(const rf_saved_activation& s) {
+  return Saved8{s.codes, s.scales, s.ld, s.scale_rows, s.format};
+}
+__device__ __forceinline__ RowView row_view_dev(const void* p, int64_t ld, int dt) {
+  return RowView{p, ld, dt, (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * (dt == RF_F32 ? 4 : 2)) % 16 == 0};
+}
+__device__ __forceinline__ RowOut row_out_dev(void* p, int64_t ld, int dt) {
+  return RowOut{p, ld, dt, (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * (dt == RF_F32 ? 4 : 2)) % 16 == 0};
+}
+// Checks of a caller's saved activation; `what` names it in the message.
+rf_status check_saved(const rf_saved_activation* s, const char* what);
+
+// -- 8 consecutive elements of a row ----------------------------------------
+// Elements at or behind `n` read as 0 and are not written.
+__device__ __forceinline__ void load8(const RowView& t, int64_t row, int64_t col, int64_t n, float (&f)[8]) {
+  if (t.vec && col + 8 <= n) {
+    if (t.dt == RF_F32) {
+      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(t.p) + row * t.ld + col);
+      const float4 a = __ldg(p), b = __ldg(p + 1);
+      f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    } else {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(t.p) + row * t.ld + col));
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      if (t.dt == RF_BF16) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          f[2 * k] = __uint_as_float(w[k] << 16);
+          f[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+          f[2 * k] = x.x;
+          f[2 * k + 1] = x.y;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = col + k < n ? ld_as_float(t.p, t.dt, row * t.ld + col + k) : 0.f;
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ void store8(const RowOut& t, int64_t row, int64_t col, int64_t n, const float (&f)[8]) {
+  if (t.vec && col + 8 <= n) {
+    if (t.dt == RF_F32) {
+      float4* p = reinterpret_cast<float4*>(static_cast<float*>(t.p) + row * t.ld + col);
+      p[0] = make_float4(f[0], f[1], f[2], f[3]);
+      p[1] = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+      uint4 u;
+      if (t.dt == RF_BF16)
+        u = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+      else
+        u = make_uint4(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]), pack_f16(f[4], f[5]), pack_f16(f[6], f[7]));
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(t.p) + row * t.ld + col) = u;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (col + k < n) st_from_float(t.p, t.dt, row * t.ld + col + k, f[k]);
+  }
+}
+
+// -- codes ------------------------------------------------------------------
+__device__ __forceinline__ float step_value(uint32_t s) {
+  return __uint_as_float(s == kNanStep ? 0x7FC00000u : s << 23);
+}
+
+// Four codes of a word -> floats (before the step).
+__device__ __forceinline__ void decode4(uint32_t w, int format, float* f) {
+  if (format == RF_INT8) {
+    // q + 128 in the low byte of 2^23's significand, then an exact subtraction.
+    const uint32_t o = w ^ 0x80808080u;
+    f[0] = __uint_as_float(__byte_perm(o, 0x4B000000u, 0x7650)) - 8388736.f;
+    f[1] = __uint_as_float(__byte_perm(o, 0x4B000000u, 0x7651)) - 8388736.f;
+    f[2] = __uint_as_float(__byte_perm(o, 0x4B000000u, 0x7652)) - 8388736.f;
+    f[3] = __uint_as_float(__byte_perm(o, 0x4B000000u, 0x7653)) - 8388736.f;
+  } else {
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(w & 0xFFFFu), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(w >> 16), __NV_E4M3);
+    const float2 x = __half22float2(__half2(a)), y = __half22float2(__half2(b));
+    f[0] = x.x, f[1] = x.y, f[2] = y.x, f[3] = y.y;
+  }
+}
+
+__device__ __forceinline__ int64_t scale_index(const Saved8& s, int64_t row, int64_t col) {
+  return ((col / kPanel8) * s.scale_rows + row) * 4 + (col % kPanel8) / kBlock8;
+}
+
+// 8 values of a saved row; zeros at and behind column s.ld (col % 8 == 0).
+__device__ __forceinline__ void load8(const Saved8& s, int64_t row, int64_t col, float (&f)[8]) {
+  if (col >= s.ld) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = 0.f;
+    return;
+  }
+  const uint2 w = __ldg(reinterpret_cast<const uint2*>(s.codes + row * s.ld + col));
+  const float st = step_value(__ldg(s.scales + scale_index(s, row, col)));
+  decode4(w.x, s.format, f);
+  decode4(w.y, s.format, f + 4);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] *= st;
+}
+
+// The step byte for a block whose largest magnitude has the float bits `a`
+// (0x7F800000 and above: not finite).
+__device__ __forceinline__ uint32_t step_byte(uint32_t a, int format) {
+  if (a >= 0x7F800000u) return kNanStep;
+  const int sh = format == RF_INT8 ? 6 : 8;
+  const uint32_t border = format == RF_INT8 ? 0x7E0000u : 0x600000u;  // significands of 127 / 64 and 448 / 256
+  const int top = format == RF_INT8 ? 248 : 246;
+  const int s = int(a >> 23) - sh + ((a & 0x7FFFFFu) > border ? 1 : 0);
+  return uint32_t(min(max(s, 1), top));
+}
+
+// Largest magnitude over a block: 8 values here, 4 neighbouring lanes in all.
+// As unsigned integers the magnitudes' bits order like the magnitudes, and an
+// infinity or a NaN is above every finite value.
+__device__ __forceinline__ uint32_t block_max_bits(const float (&f)[8]) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) a = max(a, __float_as_uint(f[k]) & 0x7FFFFFFFu);
+  a = max(a, __shfl_xor_sync(0xFFFFFFFFu, a, 1));
+  return max(a, __shfl_xor_sync(0xFFFFFFFFu, a, 2));
+}
+
+// 8 values -> 8 codes under step byte s, to nearest even.
+__device__ __forceinline__ uint2 encode8(const float (&f)[8], uint32_t s, int format) {
+  if (s == kNanStep) return make_uint2(0u, 0u);
+  const float inv = __uint_as_float((254u - s) << 23);
+  uint32_t w[2];
+  if (format == RF_INT8) {
+    uint32_t b[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)  // adding 1.5 * 2^23 rounds to an integer, whose low byte is the code
+      b[k] = __float_as_uint(fminf(fmaxf(f[k] * inv, -127.f), 127.f) + 12582912.f);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      w[h] = __byte_perm(__byte_perm(b[4 * h], b[4 * h + 1], 0x0040), __byte_perm(b[4 * h + 2], b[4 * h + 3], 0x0040),
+                         0x5410);
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * h] * inv, f[4 * h + 1] * inv), __NV_SATFINITE,
+                                                   __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * h + 2] * inv, f[4 * h + 3] * inv),
+                                                   __NV_SATFINITE, __NV_E4M3);
+      w[h] = lo | (hi << 16);
+    }
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// Writes a block quarter: the codes, and by the quad's first lane the step.
+// All 4 lanes of a quad call with consecutive columns; col < panels * 128.
+__device__ __forceinline__ void store_saved(const Saved8& s, int64_t row, int64_t col, uint2 codes, uint32_t step) {
+  if (col < s.ld) *reinterpret_cast<uint2*>(s.codes + row * s.ld + col) = codes;
+  if ((col & (kBlock8 - 1)) == 0) s.scales[scale_index(s, row, col)] = uint8_t(step);
+}
+
+// One vector of a row held by a team of whole warps, to nearest even; columns
+// behind the last panel only take part in the shuffles.
+__device__ __forceinline__ void save_row8(const Saved8& s, int64_t row, int64_t col, int64_t n, const float (&f)[8]) {
+  const uint32_t st = step_byte(block_max_bits(f), s.format);
+  if (col < (n + kPanel8 - 1) / kPanel8 * kPanel8) store_saved(s, row, col, encode8(f, st, s.format), st);
+}
+
+// A float16 array has no value above 65504; a step of the 8-bit form may.
+__device__ __forceinline__ void saturate8(int dt, float (&f)[8]) {
+  if (dt != RF_F16) return;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] = f[k] != f[k] ? f[k] : fminf(fmaxf(f[k], -65504.f), 65504.f);
+}
+
+__device__ __forceinline__ int64_t round_up_dev(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+// The value that a float holds once stored as `dt`.
+__device__ __forceinline__ void round8(int dt, float (&f)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] = round_to(dt, f[k]);
+}
+
+}  // namespace rf
