@@ -128,6 +128,73 @@ __device__ __forceinline__ void store8(const RowOut& t, int64_t row, int64_t col
   }
 }
 
+// -- typed rows on 16-byte boundaries ------------------------------------------
+// 8 elements as they lie in memory, so that the next tile's loads can be in
+// flight in few registers while this one is worked on.
+template <int DT>
+struct Raw8 {
+  uint4 u[DT == RF_F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load_raw(const void* p, int64_t i) {
+  Raw8<DT> r;
+  if (DT == RF_F32) {
+    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + i);
+    r.u[0] = __ldg(q);
+    r.u[DT == RF_F32 ? 1 : 0] = __ldg(q + 1);
+  } else {
+    r.u[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i));
+  }
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ Raw8<DT> zero_raw() {
+  Raw8<DT> r;
+  r.u[0] = make_uint4(0, 0, 0, 0);
+  r.u[DT == RF_F32 ? 1 : 0] = make_uint4(0, 0, 0, 0);
+  return r;
+}
+template <int DT>
+__device__ __forceinline__ void unpack(const Raw8<DT>& r, float (&f)[8]) {
+  const uint32_t w[4] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w};
+  if (DT == RF_F32) {
+    const uint4 v = r.u[DT == RF_F32 ? 1 : 0];
+    const uint32_t z[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f[k] = __uint_as_float(w[k]);
+      f[4 + k] = __uint_as_float(z[k]);
+    }
+  } else if (DT == RF_BF16) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f[2 * k] = __uint_as_float(w[k] << 16);
+      f[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+      f[2 * k] = x.x;
+      f[2 * k + 1] = x.y;
+    }
+  }
+}
+template <int DT>
+__device__ __forceinline__ void store_vec(void* p, int64_t i, const float (&f)[8]) {
+  if (DT == RF_F32) {
+    float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+    q[0] = make_float4(f[0], f[1], f[2], f[3]);
+    q[1] = make_float4(f[4], f[5], f[6], f[7]);
+  } else if (DT == RF_BF16) {
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) =
+        make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) =
+        make_uint4(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]), pack_f16(f[4], f[5]), pack_f16(f[6], f[7]));
+  }
+}
+
 // -- codes ------------------------------------------------------------------
 __device__ __forceinline__ float step_value(uint32_t s) {
   return __uint_as_float(s == kNanStep ? 0x7FC00000u : s << 23);
@@ -198,9 +265,14 @@ __device__ __forceinline__ uint2 encode8(const float (&f)[8], uint32_t s, int fo
   uint32_t w[2];
   if (format == RF_INT8) {
     uint32_t b[8];
+    if (s == 248u) {  // the largest step: larger magnitudes saturate
 #pragma unroll
-    for (int k = 0; k < 8; ++k)  // adding 1.5 * 2^23 rounds to an integer, whose low byte is the code
-      b[k] = __float_as_uint(fminf(fmaxf(f[k] * inv, -127.f), 127.f) + 12582912.f);
+      for (int k = 0; k < 8; ++k) b[k] = __float_as_uint(fminf(fmaxf(f[k] * inv, -127.f), 127.f) + 12582912.f);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)  // adding 1.5 * 2^23 rounds to an integer, whose low byte is the code
+        b[k] = __float_as_uint(fmaf(f[k], inv, 12582912.f));
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
       w[h] = __byte_perm(__byte_perm(b[4 * h], b[4 * h + 1], 0x0040), __byte_perm(b[4 * h + 2], b[4 * h + 3], 0x0040),

@@ -74,11 +74,15 @@ __device__ __forceinline__ float decay_term(int rdt, float decay, float p) {
 // noise is the SplitMix64 sequence (Steele, Lea and Flood, "Fast splittable
 // pseudorandom number generators", 2014) of a per-leaf seed: output c serves
 // elements 4c..4c+3, 16 bits each from the low end.
-__device__ __forceinline__ uint64_t splitmix64_at(uint64_t seed, uint64_t c) {
-  uint64_t z = seed + (c + 1) * 0x9E3779B97F4A7C15ull;
+constexpr uint64_t kSplitmixGamma = 0x9E3779B97F4A7C15ull;
+// Output of the state z = seed + (c + 1) gamma.
+__device__ __forceinline__ uint64_t splitmix64_mix(uint64_t z) {
   z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
   z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
   return z ^ (z >> 31);
+}
+__device__ __forceinline__ uint64_t splitmix64_at(uint64_t seed, uint64_t c) {
+  return splitmix64_mix(seed + (c + 1) * kSplitmixGamma);
 }
 
 __device__ __forceinline__ float sr_bf16(float x, uint32_t noise16) {

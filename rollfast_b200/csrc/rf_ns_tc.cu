@@ -535,14 +535,6 @@ struct Tc2Params {
   uint32_t idesc;
 };
 
-__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar_cluster, int c0,
-                                                 int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
 // Tile index -> (matrix, 256-row block I, 256-column block J), in an order
 // that keeps the ~one wave of tiles in flight on a few operand panels, so
 // that they share them in L2 as they advance through K together

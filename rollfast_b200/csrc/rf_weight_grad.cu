@@ -1,23 +1,36 @@
-// Weight gradient X^T G read straight from an activation saved in 8 bits.
+// Weight gradient X^T G from an activation saved in 8 bits.
 //
 //   out[i][o] = initial[i][o] + sum_t X[t][i] G[t][o]    (or its transpose)
 //
 // X [T][K] is the saved activation (rf_act8.cuh), G [T][N] the gradient of
-// the product's output.  The sum runs over tokens, along which both operands
-// are strided, so both are MN-major tensor-core operands, and the block steps
-// of X differ along the sum, so they cannot be applied to the accumulator: X
-// is turned into bfloat16 on its way to shared memory, which is exact because
-// the steps are powers of two.  The 16-bit copy of X never exists in memory.
+// the product's output.  Bound by the tensor cores (2 T K N operations).
 //
-// One persistent CTA pair (cluster of 2, tcgen05 cta_group::2) per 256 x 256
-// output tile; each CTA brings 128 rows of one operand and 128 columns of the
-// other, 64 tokens at a time:
-//   warp 0      TMA: 64 x 128 codes, their 256 bytes of steps, and 64 x 128
-//               of G (two 128-byte swizzled boxes) into a ring of kLoads
-//   warp 1      the leader's lane 0 issues tcgen05.mma (M = N = 256, K = 16)
-//   warps 2..5  epilogue: accumulator -> memory, while the next tile's
-//               products run into the other half of TMEM
-//   warps 6..9  codes -> bfloat16, into a ring of kOperands swizzled buffers
+// Operands.  The steps of X differ along the sum, so they cannot be applied
+// to the accumulator; X is expanded to bfloat16 once, in the workspace, which
+// is exact because the steps are powers of two.  Converting in the product
+// kernel instead, on the way to shared memory, was built and measured: every
+// column block converts X again, and the 2.5 instructions per element do not
+// fit beside the products (8192 x 4096 x 4096: 321 us against 210).  The
+// copy costs 346 / N of the product's time.  Float16 and float32 gradients
+// become two or three bfloat16 terms that add up to them.
+//
+// 8192 x 4096 x 14336, bfloat16 gradient, float32 result: 621 us with the
+// expansion, 1.55 PFLOP/s, 0.93 of the measured cuBLAS peak in a burst.
+//
+// Products.  One persistent CTA pair (cluster of 2, tcgen05 cta_group::2) per
+// 256 x 256 output tile; each CTA brings 128 rows of one operand and 128
+// columns of the other, 64 tokens a step.  The sum runs over rows of both
+// arrays, so both operands are MN-major:
+//   warps 0, 2   TMA: boxes of 128 tokens x 64 columns (128-byte swizzle) into a
+//                ring of kStages
+//   warp 1       the leader's lane 0 issues tcgen05.mma (M = N = 256, K = 16)
+//   warps 4..11  accumulators -> registers -> memory
+// Accuracy.  The tensor cores truncate when they add to the accumulator: over
+// 8192 tokens that left a relative error of 2.8e-6, five times that of float32
+// additions.  So the accumulator is closed every kSegment steps (1024 tokens:
+// 3.7e-7), and the epilogue warps add the segments in float32 registers (128
+// per thread) while the next segment runs into the other half of TMEM.
+//
 // Few tiles: the tokens are split over several units whose float32 partial
 // tiles a second kernel adds in a fixed order.
 #include <algorithm>
@@ -34,67 +47,72 @@ using namespace rf::tc;
 
 constexpr int kTile = 256;          // output tile of a CTA pair, both ways
 constexpr int kHalf = 128;          // operand rows per CTA
-constexpr int kTokens = 64;         // tokens per step
-constexpr int kLoads = 6;           // ring of loaded tiles
-constexpr int kOperands = 3;        // ring of converted tiles
-constexpr int kGradBytes = kTokens * kHalf * 2;
-constexpr int kCodeBytes = kTokens * kHalf;
-constexpr int kStepBytes = kTokens * 4;
-constexpr int kLoadBytes = kGradBytes + kCodeBytes + kStepBytes;
+// Tokens per step.  A step costs the issuing thread a wait and a commit beside
+// its products; with 64 tokens that thread, not the tensor cores, was the
+// bound (8192 x 4096 x 14336: 771 us against 650).
+constexpr int kTokens = 128;
+constexpr int kSegment = 8;         // steps per accumulator
+constexpr int kStages = 3;
 constexpr int kOperandBytes = kTokens * kHalf * 2;
-constexpr int kConvertWarps = 4;
-constexpr int kThreads = (6 + kConvertWarps) * 32;
-constexpr int kStagingBytes = 4 * 32 * 33 * 4;
-constexpr int kGradOff = 0;
-constexpr int kOperandOff = kGradOff + kLoads * kGradBytes;
-constexpr int kCodeOff = kOperandOff + kOperands * kOperandBytes;
-constexpr int kStepOff = kCodeOff + kLoads * kCodeBytes;
-constexpr int kStagingOff = kStepOff + kLoads * kStepBytes;
-constexpr int kBarOff = kStagingOff + kStagingBytes;
+constexpr int kBlockBytes = kTokens * 128;  // 64 columns of an operand
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kFirstEpilogue = 4, kEpilogueWarps = 8;  // a multiple of 4: a warp reads TMEM lanes 32 (warp % 4) ..
+constexpr int kThreads = (kFirstEpilogue + kEpilogueWarps) * 32;
+constexpr int kColumns = kTile / (kEpilogueWarps / 4);  // accumulator columns per epilogue warp
+constexpr int kStagingFloats = 32 * 16;                 // a warp's 32 x 16 block on its way out
+constexpr int kStagingOff = kStages * kStageBytes;
+constexpr int kBarOff = kStagingOff + kEpilogueWarps * kStagingFloats * 4;
 constexpr int kSmemBytes = kBarOff + 256 + 1024;
 static_assert(kSmemBytes <= 232448, "dynamic shared memory per CTA is at most 227 KB");
 constexpr uint32_t kTmemCols = 512;
 
 struct Params {
-  const uint8_t* scales;   // steps of X
-  int64_t scale_rows;
   int64_t m, n;            // output rows and columns
-  int64_t rows;            // tokens
-  int64_t units;           // tiles x splits
+  int64_t units;           // whole tiles, then the splits of the tail's tiles
+  int64_t whole;           // tiles computed by one unit
   int tiles_i, tiles_j;    // 256-row and 256-column blocks
-  int splits;              // units per tile
-  int steps;               // 64-token steps of all tokens
+  int splits;              // units per tile of the tail
+  int steps;               // 128-token steps of all tokens
   int terms;               // bfloat16 terms of G (1, 2 or 3)
   int x_first;             // X is the row operand (out is [K][N]), else the column operand
-  int panels;              // panels of steps
-  int format;
   const void* initial;     // added when there is one unit per tile
   void* out;
   int64_t ld_out;
   int out_dt;
-  float* partial;          // [splits][m][ld_partial] when splits > 1
-  int64_t ld_partial;
+  int vec;                 // 4 columns of out and initial can be read and written at once
+  float* partial;          // [tail tile][split][256][256]
   uint32_t idesc;
   int* error;              // the device's error word, may be null
 };
 
-// Unit -> (row block, column block, split).  All splits of a tile are
-// neighbours; tiles go down the row blocks in groups of 8 so that the ~74 in
-// flight share their operands' panels in L2.
-__device__ __forceinline__ void decode_unit(const Params& P, int64_t u, int& I, int& J, int& s) {
-  s = int(u % P.splits);
-  const int t = int(u / P.splits);
-  const int G = 8;
-  const int grp = t / (G * P.tiles_j);
+// Tile -> (row block, column block): down the row blocks in groups of 8, so
+// that the ~74 tiles in flight share their operands' panels in L2.
+__host__ __device__ __forceinline__ void tile_at(int64_t tile, int tiles_i, int tiles_j, int& I, int& J) {
+  const int t = int(tile), G = 8;
+  const int grp = t / (G * tiles_j);
   const int first = grp * G;
-  const int gm = min(P.tiles_i - first, G);
-  const int r = t - grp * G * P.tiles_j;
+  const int gm = tiles_i - first < G ? tiles_i - first : G;
+  const int r = t - grp * G * tiles_j;
   I = first + r % gm;
   J = r / gm;
 }
-__device__ __forceinline__ void split_range(const Params& P, int s, int& k0, int& k1) {
-  k0 = int(int64_t(P.steps) * s / P.splits);
-  k1 = int(int64_t(P.steps) * (s + 1) / P.splits);
+// A unit's tile, its steps [k0, k1) of the tokens, each taken once per term
+// of G, and its partial tile (-1: it writes the output itself).
+__device__ __forceinline__ void decode_unit(const Params& P, int64_t u, int& I, int& J, int& k0, int& k1,
+                                            int64_t& part) {
+  int64_t tile = u;
+  part = -1;
+  k0 = 0;
+  k1 = P.steps;
+  if (u >= P.whole) {
+    const int64_t v = u - P.whole;
+    const int s = int(v % P.splits);
+    tile = P.whole + v / P.splits;
+    if (P.splits > 1) part = v;
+    k0 = int(int64_t(P.steps) * s / P.splits);
+    k1 = int(int64_t(P.steps) * (s + 1) / P.splits);
+  }
+  tile_at(tile, P.tiles_i, P.tiles_j, I, J);
 }
 
 __device__ __forceinline__ void record_error(const Params& P, int code, volatile int* abort_flag) {
@@ -102,76 +120,91 @@ __device__ __forceinline__ void record_error(const Params& P, int code, volatile
   if (P.error) atomicCAS(P.error, 0, code);
 }
 
-__device__ __forceinline__ uint32_t bf2_mul(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r =
-      __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
+// 4 consecutive columns at element i of the output's array `initial`.
+__device__ __forceinline__ float4 initial4(const Params& P, int64_t i) {
+  if (P.out_dt == RF_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(P.initial) + i);
+  const uint2 a = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(P.initial) + i);
+  if (P.out_dt == RF_BF16)
+    return make_float4(__uint_as_float(a.x << 16), __uint_as_float(a.x & 0xFFFF0000u), __uint_as_float(a.y << 16),
+                       __uint_as_float(a.y & 0xFFFF0000u));
+  const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&a.x));
+  const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&a.y));
+  return make_float4(lo.x, lo.y, hi.x, hi.y);
 }
-__device__ __forceinline__ uint32_t bf2_sub(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r =
-      __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ void put4(const Params& P, int64_t i, float4 v) {
+  if (P.out_dt == RF_F32)
+    *reinterpret_cast<float4*>(static_cast<float*>(P.out) + i) = v;
+  else
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.out) + i) =
+        P.out_dt == RF_BF16 ? make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w))
+                            : make_uint2(pack_f16(v.x, v.y), pack_f16(v.z, v.w));
 }
-
-// Four codes -> four bfloat16 (two words), times the step; every operation is
-// exact.  int8: with b the byte, 0x4300 | (b & 0x7F) is 128 + (b & 0x7F) and
-// 0x4300 | (b & 0x80) is 128 or 256, so their difference is the code.  e4m3:
-// its exponent and significand in bfloat16's places stand for 2^-120 of the
-// value (subnormals too).
-template <int kFormat>
-__device__ __forceinline__ void convert4(uint32_t w, uint32_t step2, uint32_t& lo, uint32_t& hi) {
-  if (kFormat == RF_INT8) {
-    const uint32_t a = __byte_perm(w, 0x43434343u, 0x4140), b = __byte_perm(w, 0x43434343u, 0x4342);
-    lo = bf2_mul(bf2_sub(a & 0xFF7FFF7Fu, a & 0xFF80FF80u), step2);
-    hi = bf2_mul(bf2_sub(b & 0xFF7FFF7Fu, b & 0xFF80FF80u), step2);
-  } else {
-    const uint32_t a = __byte_perm(w, 0u, 0x1404), b = __byte_perm(w, 0u, 0x3424);
-    const uint32_t k2p120 = 0x7B807B80u;
-    lo = bf2_mul(bf2_mul((a & 0x80008000u) | ((a >> 4) & 0x07F007F0u), k2p120), step2);
-    hi = bf2_mul(bf2_mul((b & 0x80008000u) | ((b >> 4) & 0x07F007F0u), k2p120), step2);
+// The same without vectors, `live` of the columns.
+__device__ __forceinline__ void add_put_each(const Params& P, int64_t i, int64_t live, float4 v) {
+  const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (k >= live) break;
+    float x = f[k];
+    if (P.initial) x += ld_as_float(P.initial, P.out_dt, i + k);
+    st_from_float(P.out, P.out_dt, i + k, x);
   }
 }
+__device__ __forceinline__ float4 add4(float4 a, float4 b) {
+  return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+}
 
-// One 32 x 32 block of the output, lane = row in v[], through the warp's
-// staging buffer so that a store covers a row's 32 columns.
-__device__ __forceinline__ void store_block(const Params& P, int split, int64_t row0, int64_t col0, int lane,
+// A warp's 32 x 16 block, lane = row in v[], through its staging buffer, so
+// that a store instruction covers 8 rows of 64 bytes.  16-byte chunk c of row
+// r lies at c ^ (r / 2 % 4): both the row writes and the reads of 8 rows by 4
+// chunks touch every bank once.  The initial values of a block are loaded
+// together, ahead of their use: one at a time, their latency outlasted the
+// next tile's products.
+__device__ __forceinline__ void store_block(const Params& P, float* part, int64_t row0, int64_t col0, int lane,
                                             const float* v, float* stg) {
+  const int r0 = lane >> 2;
+  const int64_t col = col0 + 4 * (lane & 3);
+  const int64_t live = P.n - col;
+  const bool vec = P.vec && live >= 4;
+  const int64_t ld = part ? kTile : P.ld_out;
+  const int64_t i = part ? (row0 + r0) % kTile * kTile + col % kTile : (row0 + r0) * P.ld_out + col;
+  const int rows = int(min(P.m - row0 - r0, int64_t(32)));  // this lane's row r0 + 8 it is inside while 8 it < rows
+  float4 a[4];
+#pragma unroll
+  for (int it = 0; it < 4; ++it) {
+    a[it] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!part && P.initial && vec && 8 * it < rows) a[it] = initial4(P, i + 8 * it * ld);
+  }
   __syncwarp();
 #pragma unroll
-  for (int k = 0; k < 32; ++k) stg[lane * 33 + k] = v[k];
+  for (int c = 0; c < 4; ++c)
+    *reinterpret_cast<float4*>(stg + lane * 16 + ((c ^ ((lane >> 1) & 3)) << 2)) =
+        make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
   __syncwarp();
-  const int64_t col = col0 + lane;
-  if (col >= P.n) return;
-  const int rows = int(P.m - row0 < 32 ? P.m - row0 : 32);
-  if (P.splits > 1) {
-    float* o = P.partial + (int64_t(split) * P.m + row0) * P.ld_partial + col;
-    for (int r = 0; r < rows; ++r) o[int64_t(r) * P.ld_partial] = stg[r * 33 + lane];
-  } else {
-    const int64_t base = row0 * P.ld_out + col;
-#pragma unroll 4
-    for (int r = 0; r < rows; ++r) {
-      float x = stg[r * 33 + lane];
-      const int64_t i = base + int64_t(r) * P.ld_out;
-      if (P.initial) x += ld_as_float(P.initial, P.out_dt, i);
-      st_from_float(P.out, P.out_dt, i, x);
-    }
+  if (live <= 0) return;
+  // Row r0 + 8 it: r / 2 % 4 is that of r0.
+  const float* src = stg + r0 * 16 + (((lane & 3) ^ ((r0 >> 1) & 3)) << 2);
+#pragma unroll
+  for (int it = 0; it < 4; ++it) {
+    if (8 * it >= rows) break;
+    const float4 x = *reinterpret_cast<const float4*>(src + 128 * it);
+    if (part) *reinterpret_cast<float4*>(part + i + 8 * it * ld) = x;
+    else if (vec) put4(P, i + 8 * it * ld, add4(x, a[it]));
+    else add_put_each(P, i + 8 * it * ld, live, x);
   }
 }
 
-template <int kFormat>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    k_weight_grad(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_grad,
+    k_weight_grad(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_g,
                   const __grid_constant__ Params P) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBarOff);
-  const uint32_t full0 = smem_u32(bars);                       // loads landed (own CTA)
-  const uint32_t empty0 = full0 + 8 * kLoads;                  // loads consumed (commit, both CTAs)
-  const uint32_t ready0 = empty0 + 8 * kLoads;                 // operand converted (leader: both CTAs' warps)
-  const uint32_t free0 = ready0 + 8 * kOperands;               // operand consumed (commit, both CTAs)
-  const uint32_t accf0 = free0 + 8 * kOperands;                // accumulator complete
-  const uint32_t acce0 = accf0 + 16;                           // accumulator read (leader: both CTAs' warps)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kLoads + 2 * kOperands + 4);
+  const uint32_t full0 = smem_u32(bars);              // loads landed (the leader's: both CTAs')
+  const uint32_t empty0 = full0 + 8 * kStages;        // loads consumed (commit, both CTAs)
+  const uint32_t accf0 = empty0 + 8 * kStages;        // accumulator complete (commit, both CTAs)
+  const uint32_t acce0 = accf0 + 16;                  // accumulator read (leader: both CTAs' warps)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
@@ -179,17 +212,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int64_t pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kLoads; ++s) {
-      mbar_init(full0 + 8 * s, 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full0 + 8 * s, 2);
       mbar_init(empty0 + 8 * s, 1);
-    }
-    for (int s = 0; s < kOperands; ++s) {
-      mbar_init(ready0 + 8 * s, 2 * kConvertWarps);
-      mbar_init(free0 + 8 * s, 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(accf0 + 8 * s, 1);
-      mbar_init(acce0 + 8 * s, 8);
+      mbar_init(acce0 + 8 * s, 2 * kEpilogueWarps);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -204,37 +233,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0) {
+  if (warp < kFirstEpilogue) {
+  // Registers move to the epilogue's sums: 72 + 2 x 216 of the launch's 3 x 168.
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  if (warp == 0 || warp == 2) {
     if (lane == 0) {
       // ---------------- loads (both CTAs, each its own halves) ----------------
+      // A warp for each operand: a wait and four copies take one thread about
+      // as long as the products of a step.
+      const bool x = warp == 0;
+      const CUtensorMap* map = x ? &tm_x : &tm_g;
       int stage = 0;
       uint32_t phase = 0;
       int64_t fills = 0;
       bool ok = true;
       for (int64_t u = pair; ok && u < P.units; u += npairs) {
-        int I, J, s, k0, k1;
-        decode_unit(P, u, I, J, s);
-        split_range(P, s, k0, k1);
-        const int xcol = (P.x_first ? I : J) * kTile + int(rank) * kHalf;
-        const int gcol = (P.x_first ? J : I) * kTile + int(rank) * kHalf;
-        const int panel = min(xcol / kPanel8, P.panels - 1);  // columns behind the last read zeros under any step
-        for (int k = k0; ok && k < k1; ++k) {
-          for (int term = 0; term < P.terms; ++term) {
-            if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, abort_flag)) {
+        int I, J, k0, k1;
+        int64_t part;
+        decode_unit(P, u, I, J, k0, k1, part);
+        const int col = ((P.x_first != 0) == x ? I : J) * kTile + int(rank) * kHalf;
+        // The smallest term first: what the accumulator's truncation costs
+        // goes with its magnitude, which only the last pass brings up.
+        for (int term = P.terms - 1; ok && term >= 0; --term) {
+          for (int k = k0; k < k1; ++k) {
+            if (!mbar_wait_short(empty0 + 8 * stage, phase ^ 1, abort_flag)) {
               record_error(P, kDevTimeoutProducer, abort_flag);
               ok = false;
               break;
             }
-            const uint32_t fb = full0 + 8 * stage;
-            mbar_arrive_expect_tx(fb, kLoadBytes);
-            const uint32_t g = smem_u32(smem + kGradOff + stage * kGradBytes);
-            tma_load_2d(smem_u32(smem + kCodeOff + stage * kCodeBytes), &tm_codes, fb, xcol, k * kTokens);
-            bulk_load(smem_u32(smem + kStepOff + stage * kStepBytes),
-                      P.scales + (int64_t(panel) * P.scale_rows + int64_t(k) * kTokens) * 4, fb, kStepBytes);
-            tma_load_3d(g, &tm_grad, fb, gcol, k * kTokens, term);
-            tma_load_3d(g + 8192, &tm_grad, fb, gcol + 64, k * kTokens, term);
+            // Both CTAs' copies complete on the leader's barrier.
+            if (leader) mbar_arrive_expect_tx(full0 + 8 * stage, 2 * kOperandBytes);
+            const uint32_t fb = map_to_rank(full0 + 8 * stage, 0);
+            const uint32_t dst = smem_u32(smem + stage * kStageBytes) + (x ? 0 : kOperandBytes);
+            tma_load_3d_pair(dst, map, fb, col, k * kTokens, x ? 0 : term);
+            tma_load_3d_pair(dst + kBlockBytes, map, fb, col + 64, k * kTokens, x ? 0 : term);
             ++fills;
-            if (++stage == kLoads) {
+            if (++stage == kStages) {
               stage = 0;
               phase ^= 1;
             }
@@ -243,154 +277,122 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       // The last fills have been consumed: no copy into this CTA and no
       // commit's arrival on these barriers is pending.
-      for (int64_t f = fills > kLoads ? fills - kLoads : 0; f < fills; ++f)
-        mbar_drain(empty0 + 8 * uint32_t(f % kLoads), uint32_t((f / kLoads) & 1));
+      for (int64_t f = fills > kStages ? fills - kStages : 0; f < fills; ++f)
+        mbar_drain(empty0 + 8 * uint32_t(f % kStages), uint32_t((f / kStages) & 1));
     }
   } else if (warp == 1) {
     if (lane == 0 && leader) {
       // ---------------- products ----------------
-      int stage = 0, buf = 0;
-      uint32_t bphase = 0;
+      const uint32_t ring = smem_u32(smem);
+      const uint64_t xd = sdesc(ring, kBlockBytes, 1024), gd = sdesc(ring + kOperandBytes, kBlockBytes, 1024);
+      const uint64_t ad = P.x_first ? xd : gd, bd = P.x_first ? gd : xd;
+      int stage = 0;
+      uint32_t phase = 0;
       int acc = 0;
       uint32_t acc_phase = 0;
       bool ok = true;
-      int tiles_done = 0;
+      int64_t segments = 0;
+      uint32_t loaded = 0;  // the current stage's loads were seen complete
       for (int64_t u = pair; ok && u < P.units; u += npairs) {
-        int I, J, s, k0, k1;
-        decode_unit(P, u, I, J, s);
-        split_range(P, s, k0, k1);
-        if (!mbar_wait_cluster(acce0 + 8 * acc, acc_phase ^ 1, abort_flag)) {
-          record_error(P, kDevTimeoutMma, abort_flag);
-          break;
-        }
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + uint32_t(acc * kTile);
+        int I, J, k0, k1;
+        int64_t part;
+        decode_unit(P, u, I, J, k0, k1, part);
         const int n_steps = (k1 - k0) * P.terms;
-        for (int k = 0; k < n_steps; ++k) {
-          if (!mbar_wait_cluster(ready0 + 8 * buf, bphase, abort_flag)) {
+        for (int b = 0; ok && b < n_steps; b += kSegment) {
+          if (!mbar_wait_short(acce0 + 8 * acc, acc_phase ^ 1, abort_flag)) {
             record_error(P, kDevTimeoutMma, abort_flag);
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t g = smem_u32(smem + kGradOff + stage * kGradBytes);
-          const uint32_t x = smem_u32(smem + kOperandOff + buf * kOperandBytes);
-          const uint32_t sa = P.x_first ? x : g, sb = P.x_first ? g : x;
+          const uint32_t d_tmem = tmem_base + uint32_t(acc * kTile);
+          const int e = min(b + kSegment, n_steps);
+          for (int k = b; k < e; ++k) {
+            if (!loaded && !mbar_wait_short(full0 + 8 * stage, phase, abort_flag)) {
+              record_error(P, kDevTimeoutMma, abort_flag);
+              ok = false;
+              break;
+            }
+            const uint32_t now = uint32_t(stage);
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1;
+            }
+            loaded = mbar_test(full0 + 8 * stage, phase);
+            tc_fence_after();
+            // Descriptors count 16-byte units: a stage further, 16 tokens further.
+            const uint64_t off = uint64_t(now * (kStageBytes >> 4));
 #pragma unroll
-          for (int q = 0; q < kTokens / 16; ++q)
-            mma_f16_pair(d_tmem, sdesc(sa + q * 2048, 8192, 1024), sdesc(sb + q * 2048, 8192, 1024), P.idesc,
-                         (k | q) != 0);
-          mma_commit_pair(empty0 + 8 * stage);
-          mma_commit_pair(free0 + 8 * buf);
-          if (++stage == kLoads) stage = 0;
-          if (++buf == kOperands) {
-            buf = 0;
-            bphase ^= 1;
+            for (int q = 0; q < kTokens / 16; ++q)
+              mma_f16_pair(d_tmem, ad + off + q * (2048 >> 4), bd + off + q * (2048 >> 4), P.idesc,
+                           (k > b || q > 0) ? 1u : 0u);
+            mma_commit_pair(empty0 + 8 * now);
           }
+          if (!ok) break;
+          mma_commit_pair(accf0 + 8 * acc);
+          ++segments;
+          acc ^= 1;
+          if (acc == 0) acc_phase ^= 1;
         }
-        if (!ok) break;
-        mma_commit_pair(accf0 + 8 * acc);
-        ++tiles_done;
+      }
+      // Both CTAs' epilogues have released the last two accumulators.
+      for (int64_t k = segments > 2 ? segments - 2 : 0; k < segments; ++k)
+        mbar_drain(acce0 + 8 * uint32_t(k & 1), uint32_t((k >> 1) & 1));
+    }
+  }
+  } else {
+    // ---------------- segments -> registers -> memory (both CTAs) ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int quarter = warp & 3;                         // TMEM lanes 32 * quarter .. + 31
+    const int first_col = ((warp - kFirstEpilogue) >> 2) * kColumns;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    float* stg = reinterpret_cast<float*>(smem + kStagingOff) + (warp - kFirstEpilogue) * kStagingFloats;
+    bool ok = true;
+    for (int64_t u = pair; ok && u < P.units; u += npairs) {
+      int I, J, k0, k1;
+      int64_t part;
+      decode_unit(P, u, I, J, k0, k1, part);
+      const int n_steps = (k1 - k0) * P.terms;
+      float sum[kColumns];
+#pragma unroll
+      for (int i = 0; i < kColumns; ++i) sum[i] = 0.f;
+      for (int b = 0; b < n_steps; b += kSegment) {
+        // One lane polls, for the other waits' sake.
+        if (lane == 0) ok = mbar_wait_short(accf0 + 8 * acc, acc_phase, abort_flag);
+        ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+        if (!ok) {
+          record_error(P, kDevTimeoutEpilogue, abort_flag);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t t = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(acc * kTile + first_col);
+#pragma unroll
+        for (int c = 0; c < kColumns; c += 32) {
+          uint32_t v[2][16];
+          tmem_ld16_async(t + c, v[0]);
+          tmem_ld16_async(t + c + 16, v[1]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sum[c + i] += __uint_as_float(v[i >> 4][i & 15]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(map_to_rank(acce0 + 8 * acc, 0));
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
-      // Both CTAs' epilogues have released the last two tiles.
-      for (int k = tiles_done > 2 ? tiles_done - 2 : 0; k < tiles_done; ++k)
-        mbar_drain(acce0 + 8 * uint32_t(k & 1), uint32_t((k >> 1) & 1));
-    }
-  } else if (warp < 6) {
-    // ---------------- epilogue (both CTAs) ----------------
-    const int quarter = warp & 3;  // TMEM lanes 32 * quarter .. + 31
-    int acc = 0;
-    uint32_t acc_phase = 0;
-    float* stg = reinterpret_cast<float*>(smem + kStagingOff) + (warp - 2) * (32 * 33);
-    for (int64_t u = pair; u < P.units; u += npairs) {
-      int I, J, s;
-      decode_unit(P, u, I, J, s);
-      if (!mbar_wait(accf0 + 8 * acc, acc_phase, abort_flag)) {
-        record_error(P, kDevTimeoutEpilogue, abort_flag);
-        break;
-      }
-      tc_fence_after();
+      if (!ok) break;
       const int64_t row0 = int64_t(I) * kTile + int64_t(rank) * kHalf + quarter * 32;
-      const int64_t col0 = int64_t(J) * kTile;
-      for (int ch = 0; ch < kTile / 32; ++ch) {
-        if (row0 >= P.m || col0 + ch * 32 >= P.n) break;
-        float v[32];
-        __syncwarp();
-        tmem_ld32(tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(acc * kTile + ch * 32), v);
-        store_block(P, s, row0, col0 + ch * 32, lane, v, stg);
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_to_rank(acce0 + 8 * acc, 0));
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1;
-    }
-  } else {
-    // ---------------- codes -> bfloat16 (both CTAs) ----------------
-    const int tid = int(threadIdx.x) - 6 * 32;
-    int stage = 0, buf = 0;
-    uint32_t phase = 0, bphase = 0;
-    int64_t fills = 0;
-    bool ok = true;
-    for (int64_t u = pair; ok && u < P.units; u += npairs) {
-      int I, J, s, k0, k1;
-      decode_unit(P, u, I, J, s);
-      split_range(P, s, k0, k1);
-      for (int k = k0; ok && k < k1; ++k) {
-        for (int term = 0; term < P.terms; ++term) {
-          ok = mbar_wait(full0 + 8 * stage, phase, abort_flag) && mbar_wait(free0 + 8 * buf, bphase ^ 1, abort_flag);
-          if (!ok) {
-            record_error(P, kDevTimeoutProducer, abort_flag);
-            break;
-          }
-          const uint8_t* codes = smem + kCodeOff + stage * kCodeBytes;
-          const uint8_t* steps = smem + kStepOff + stage * kStepBytes;
-          uint8_t* dst = smem + kOperandOff + buf * kOperandBytes;
-          const int live = int(P.rows - int64_t(k) * kTokens < kTokens ? P.rows - int64_t(k) * kTokens : kTokens);
+      const int64_t col0 = int64_t(J) * kTile + first_col;
+      float* dst = part < 0 ? nullptr : P.partial + part * (kTile * kTile);
+      if (row0 < P.m) {
 #pragma unroll
-          for (int it = 0; it < kTokens * 8 / (kConvertWarps * 32); ++it) {
-            const int idx = it * (kConvertWarps * 32) + tid;
-            const int t = idx >> 3, j = idx & 7;  // token, group of 16 features
-            const uint4 c = *reinterpret_cast<const uint4*>(codes + t * kHalf + j * 16);
-            uint32_t st = steps[t * 4 + (j >> 1)];
-            // Tokens behind the last have zero codes and unwritten steps.
-            if (t >= live) st = 127u;
-            uint32_t st2 = st == kNanStep ? 0x7FC0u : st << 7;
-            st2 |= st2 << 16;
-            uint4 lo, hi;
-            convert4<kFormat>(c.x, st2, lo.x, lo.y);
-            convert4<kFormat>(c.y, st2, lo.z, lo.w);
-            convert4<kFormat>(c.z, st2, hi.x, hi.y);
-            convert4<kFormat>(c.w, st2, hi.z, hi.w);
-            // MN-major, 128-byte swizzle: 64-feature blocks of [token][128
-            // bytes], 16-byte chunk c of token t at c ^ (t & 7).  The two
-            // blocks' threads store their chunks in opposite order, so that a
-            // row's 8 stores fall on 8 different chunks.
-            uint8_t* row = dst + (j >> 2) * 8192 + t * 128;
-            const int c0 = (j & 3) * 2, sw = t & 7, odd = j >> 2;
-            *reinterpret_cast<uint4*>(row + (((c0 + odd) ^ sw) << 4)) = odd ? hi : lo;
-            *reinterpret_cast<uint4*>(row + (((c0 + 1 - odd) ^ sw) << 4)) = odd ? lo : hi;
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(map_to_rank(ready0 + 8 * buf, 0));
-          ++fills;
-          if (++stage == kLoads) {
-            stage = 0;
-            phase ^= 1;
-          }
-          if (++buf == kOperands) {
-            buf = 0;
-            bphase ^= 1;
-          }
+        for (int c = 0; c < kColumns; c += 16) {
+          if (col0 + c < P.n) store_block(P, dst, row0, col0 + c, lane, sum + c, stg);
         }
       }
     }
-    if (tid == 0)
-      for (int64_t f = fills > kOperands ? fills - kOperands : 0; f < fills; ++f)
-        mbar_drain(free0 + 8 * uint32_t(f % kOperands), uint32_t((f / kOperands) & 1));
   }
 
   __syncwarp();
@@ -429,68 +431,79 @@ __global__ void __launch_bounds__(256) k_grad_terms(RowView g, uint16_t* out, in
   }
 }
 
-// out = initial + partial[0] + partial[1] + ... in this order.
-__global__ void __launch_bounds__(256) k_weight_grad_join(const float* partial, int splits, int64_t m, int64_t n,
-                                                          int64_t ld_partial, const void* initial, void* out,
-                                                          int64_t ld_out, int out_dt) {
-  const int64_t col = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 4;
-  if (col >= n) return;
-  const int live = int(n - col < 4 ? n - col : 4);
-  for (int64_t row = int64_t(blockIdx.x) * blockDim.y + threadIdx.y; row < m; row += int64_t(gridDim.x) * blockDim.y) {
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < splits; ++s) {
-      const float4 x = *reinterpret_cast<const float4*>(partial + (int64_t(s) * m + row) * ld_partial + col);
-      a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
-    }
-    const float f[4] = {a.x, a.y, a.z, a.w};
-    const int64_t base = row * ld_out + col;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (k >= live) break;
-      float x = f[k];
-      if (initial) x += ld_as_float(initial, out_dt, base + k);
-      st_from_float(out, out_dt, base + k, x);
-    }
+// The tail's tiles: out = initial + partial[0] + partial[1] + ... in this
+// order.  A CTA takes 4 rows of a tile; without splits (no tokens) the sum is
+// 0 everywhere.
+__global__ void __launch_bounds__(256) k_weight_grad_join(const __grid_constant__ Params P) {
+  const int64_t tail = blockIdx.x / (kTile / 4);
+  const int r = int(blockIdx.x % (kTile / 4)) * 4 + int(threadIdx.x >> 6), c = int(threadIdx.x & 63) * 4;
+  int I, J;
+  tile_at(P.whole + tail, P.tiles_i, P.tiles_j, I, J);
+  const int64_t row = int64_t(I) * kTile + r, col = int64_t(J) * kTile + c;
+  if (row >= P.m || col >= P.n) return;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  const float* p = P.partial + tail * P.splits * (kTile * kTile) + r * kTile + c;
+#pragma unroll 4
+  for (int s = 0; s < P.splits; ++s) {
+    const float4 x = *reinterpret_cast<const float4*>(p + int64_t(s) * (kTile * kTile));
+    a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
   }
+  const int64_t i = row * P.ld_out + col;
+  if (!P.vec || P.n - col < 4) add_put_each(P, i, P.n - col, a);
+  else put4(P, i, P.initial ? add4(a, initial4(P, i)) : a);
 }
 
-rf_status make_map(CUtensorMap* map, CUtensorMapDataType dt, const void* base, int rank, const cuuint64_t* dims,
-                   const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+// Boxes of kTokens tokens x 64 columns over [terms][rows][cols] bfloat16, rows ld
+// elements apart (a multiple of 8); columns and tokens behind the last read 0.
+rf_status make_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t terms, int64_t ld) {
   auto fn = tensor_map_encoder();
   if (!fn) return fail(RF_ECUDA, "cuTensorMapEncodeTiled entry point unavailable");
-  const cuuint32_t ones[3] = {1, 1, 1};
-  const CUresult r = fn(map, dt, cuuint32_t(rank), const_cast<void*>(base), dims, strides, box, ones,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  const cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(terms)};
+  const cuuint64_t strides[2] = {cuuint64_t(ld) * 2, cuuint64_t(ld) * 2 * cuuint64_t(rows)};
+  const cuuint32_t box[3] = {64, kTokens, 1}, ones[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, ones,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(RF_ECUDA, "cuTensorMapEncodeTiled failed: " + std::to_string(int(r)));
   return RF_OK;
 }
 
-// Units per tile.  With at least a wave of tiles the tokens stay whole.
-// Otherwise the number that minimises a model of the time, in 64-token steps
-// of one pair: waves of units, each its steps plus about 8 steps of prologue
-// and epilogue, and the partial tiles' way through L2 (a pair moves a 256 x
-// 256 float32 tile in about 3 steps; each split adds one tile written and read).
-int choose_splits(int64_t tiles, int64_t steps, int64_t pairs) {
-  if (tiles >= pairs || steps <= 1) return 1;
-  double best = 0;
-  int split = 1;
-  for (int s = 1; s <= 64 && s * 2 <= steps; ++s) {
-    const double waves = double(ceil_div(tiles * s, pairs));
-    const double t = waves * (double(ceil_div(steps, s)) + 8) + (s > 1 ? 12 + 3.0 * double(tiles) * s / pairs : 0);
-    if (s == 1 || t < best) {
-      best = t;
-      split = s;
+// Which tiles are split over the tokens, and into how many units.  All tiles
+// that fill a wave of pairs stay whole; the rest (all, when there are fewer
+// than pairs) would leave pairs idle and are split into the number that
+// minimises a model of the remaining time, in steps of one pair: waves of
+// units, each its steps plus about 4 of prologue and epilogue, and for a split
+// the partial tiles' way through L2 (about 6 steps, and 1.5 for every tile a
+// pair has to write and read).
+struct Tail {
+  int64_t whole;
+  int splits;
+};
+Tail choose_tail(int64_t tiles, int64_t steps, int64_t pairs) {
+  Tail t{tiles - tiles % pairs, 1};
+  const int64_t rest = tiles - t.whole;
+  if (rest == 0) return t;
+  double best = double(steps) + 4;
+  for (int s = 2; s <= 64 && s * 2 <= steps; ++s) {
+    const double waves = double(ceil_div(rest * s, pairs));
+    const double cost = waves * (double(ceil_div(steps, s)) + 4) + 6 + 1.5 * double(rest * s) / double(pairs);
+    if (cost < best) {
+      best = cost;
+      t.splits = s;
     }
   }
-  return split;
+  if (t.splits == 1) t.whole = tiles;
+  return t;
 }
 
 struct Plan {
+  int64_t ld_x;         // row stride of the expanded X
   int64_t ld_terms;     // 0: G is read in place
-  size_t terms_bytes, partial_bytes;
-  int terms, splits;
-  int64_t ld_partial, steps;
+  size_t x_bytes, terms_bytes, partial_bytes;
+  int terms;
+  Tail tail;
+  int64_t steps;
+  size_t total() const { return x_bytes + terms_bytes + partial_bytes; }
 };
 
 // `in_place`: the gradient is bfloat16 and its rows start on 16-byte boundaries.
@@ -498,23 +511,19 @@ Plan make_plan(int64_t rows, int64_t features, int64_t n_out, int32_t dt, bool i
   Plan p{};
   p.terms = dt == RF_BF16 ? 1 : dt == RF_F16 ? 2 : 3;
   p.steps = ceil_div(rows, kTokens);
+  p.ld_x = round_up(features, 8);
+  p.x_bytes = align_up(size_t(rows) * size_t(p.ld_x) * 2, 256);
   if (!(dt == RF_BF16 && in_place)) {
     p.ld_terms = round_up(n_out, 8);
     p.terms_bytes = align_up(size_t(p.terms) * size_t(rows) * size_t(p.ld_terms) * 2, 256);
   }
   const int64_t tiles = ceil_div(features, kTile) * ceil_div(n_out, kTile);
-  p.splits = rows > 0 ? choose_splits(tiles, p.steps * p.terms, pairs) : 0;
-  if (p.splits > p.steps) p.splits = int(p.steps);
-  // Rows of the partial tiles are output rows, so either layout may be the
-  // longer one; both are counted with the larger padding.
-  p.ld_partial = 0;
-  if (p.splits > 1)
-    p.partial_bytes = size_t(p.splits) * 4 *
-                      size_t(std::max(features * round_up(n_out, 4), n_out * round_up(features, 4)));
+  if (rows > 0) p.tail = choose_tail(tiles, p.steps, pairs);
+  else p.tail = Tail{0, 0};
+  p.partial_bytes = size_t(tiles - p.tail.whole) * size_t(p.tail.splits) * kTile * kTile * 4;
   return p;
 }
 
-template <int kFormat>
 int64_t max_pairs() {
   static std::mutex mu;
   static int64_t cache[64] = {};
@@ -528,7 +537,7 @@ int64_t max_pairs() {
     cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = kSmemBytes;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, k_weight_grad<kFormat>, &cfg) != cudaSuccess || n <= 0) {
+    if (cudaOccupancyMaxActiveClusters(&n, k_weight_grad, &cfg) != cudaSuccess || n <= 0) {
       cudaGetLastError();
       n = num_sms() / 2;
     }
@@ -537,7 +546,6 @@ int64_t max_pairs() {
   return c;
 }
 
-template <int kFormat>
 rf_status allow_smem() {
   static std::mutex mu;
   static bool done[64] = {};
@@ -545,20 +553,10 @@ rf_status allow_smem() {
   cudaGetDevice(&dev);
   std::lock_guard<std::mutex> lk(mu);
   if (done[dev & 63]) return RF_OK;
-  const cudaError_t e =
-      cudaFuncSetAttribute(k_weight_grad<kFormat>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  const cudaError_t e = cudaFuncSetAttribute(k_weight_grad, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   if (e != cudaSuccess) return fail(RF_ECUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
   done[dev & 63] = true;
   return RF_OK;
-}
-
-template <int kFormat>
-rf_status launch(const CUtensorMap& mc, const CUtensorMap& mg, const Params& P, cudaStream_t st) {
-  RF_TRY(allow_smem<kFormat>());
-  const int64_t cap = max_pairs<kFormat>();
-  const int64_t pairs = P.units < cap ? P.units : cap;
-  k_weight_grad<kFormat><<<unsigned(2 * pairs), kThreads, kSmemBytes, st>>>(mc, mg, P);
-  return check_launch("k_weight_grad");
 }
 
 // Half the SMs: the split rule must not depend on a query that fails without
@@ -568,8 +566,9 @@ int64_t plan_pairs() { return 74; }
 rf_status check_sizes(int64_t rows, int64_t features, int64_t n_out, int32_t dt, int64_t ld) {
   if (!valid_dtype(dt)) return fail(RF_EINVAL, "rf_weight_gradient: grad dtype must be RF_F32, RF_BF16 or RF_F16");
   if (rows < 0 || rows > 0x7FFFFFFF - kTokens || features <= 0 || features > kMaxFeatures || n_out <= 0 ||
-      n_out > kMaxFeatures)
-    return fail(RF_EINVAL, "rf_weight_gradient: rows in [0, 2^31 - 64), features and n_out in [1, 2^26]");
+      n_out > kMaxFeatures || ceil_div(features, kTile) * ceil_div(n_out, kTile) > (int64_t(1) << 24))
+    return fail(RF_EINVAL, "rf_weight_gradient: rows in [0, 2^31 - 128), features and n_out in [1, 2^26], at most "
+                           "2^24 tiles of 256 x 256");
   if (ld < n_out) return fail(RF_EINVAL, "rf_weight_gradient: ld_grad below n_out");
   return RF_OK;
 }
@@ -586,7 +585,7 @@ extern "C" rf_status rf_weight_gradient_workspace_size(int64_t rows, int64_t fea
   RF_TRY(wg::check_sizes(rows, features, n_out, grad_dtype, ld_grad));
   const bool in_place = grad_dtype == RF_BF16 && rows_vectorised(grad_out, ld_grad, RF_BF16);
   const wg::Plan p = wg::make_plan(rows, features, n_out, grad_dtype, in_place, wg::plan_pairs());
-  *bytes = p.terms_bytes + p.partial_bytes;
+  *bytes = p.total();
   return RF_OK;
 }
 
@@ -610,17 +609,38 @@ extern "C" rf_status rf_weight_gradient(const rf_saved_activation* saved, const 
     return fail(RF_EINVAL, "rf_weight_gradient: misaligned pointer");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool in_place = grad_dtype == RF_BF16 && rows_vectorised(grad_out, ld_grad, RF_BF16);
-  Plan p = make_plan(rows, features, n_out, grad_dtype, in_place, plan_pairs());
-  p.ld_partial = round_up(n, 4);
-  if (p.terms_bytes + p.partial_bytes > workspace_bytes)
-    return fail(RF_EINVAL, "rf_weight_gradient: workspace too small: " +
-                               std::to_string(p.terms_bytes + p.partial_bytes) + " bytes needed");
-  if (p.terms_bytes + p.partial_bytes > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256))
+  const Plan p = make_plan(rows, features, n_out, grad_dtype, in_place, plan_pairs());
+  if (p.total() > workspace_bytes)
+    return fail(RF_EINVAL, "rf_weight_gradient: workspace too small: " + std::to_string(p.total()) + " bytes needed");
+  if (p.total() > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256))
     return fail(RF_EINVAL, "rf_weight_gradient: the workspace must be 256-byte aligned");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  float* partial = reinterpret_cast<float*>(ws + p.terms_bytes);
+
+  Params P{};
+  P.m = m;
+  P.n = n;
+  P.tiles_i = int(ceil_div(m, kTile));
+  P.tiles_j = int(ceil_div(n, kTile));
+  const int64_t tiles = int64_t(P.tiles_i) * P.tiles_j;
+  P.whole = p.tail.whole;
+  P.splits = p.tail.splits;
+  P.units = P.whole + (tiles - P.whole) * P.splits;
+  P.steps = int(p.steps);
+  P.terms = p.terms;
+  P.x_first = layout == RF_IN_OUT;
+  P.initial = initial;
+  P.out = out;
+  P.ld_out = ld_out;
+  P.out_dt = out_dtype;
+  P.vec = ld_out % 4 == 0 && (reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(initial)) % (4 * oes) == 0;
+  P.partial = reinterpret_cast<float*>(ws + p.x_bytes + p.terms_bytes);
+  P.error = device_error_word();
+  // bfloat16 operands, float32 accumulator, both operands MN-major.
+  P.idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | (uint32_t(kTile >> 3) << 17) |
+            (uint32_t(kTile >> 4) << 24);
 
   if (rows > 0) {
+    RF_TRY(rf_load_activation(saved, ws, p.ld_x, RF_BF16, stream));
     const void* g = grad_out;
     int64_t ldg = ld_grad;
     if (p.ld_terms) {
@@ -628,51 +648,21 @@ extern "C" rf_status rf_weight_gradient(const rf_saved_activation* saved, const 
       const int tx = int(nv < 256 ? nv : 256), ty = 256 / tx;
       const int64_t gx = std::min<int64_t>(ceil_div(rows, ty), 65535);
       k_grad_terms<<<dim3(unsigned(gx), unsigned(ceil_div(nv, tx))), dim3(unsigned(tx), unsigned(ty)), 0, st>>>(
-          row_view(grad_out, ld_grad, grad_dtype), reinterpret_cast<uint16_t*>(ws), rows, n_out, p.ld_terms, p.terms);
+          row_view(grad_out, ld_grad, grad_dtype), reinterpret_cast<uint16_t*>(ws + p.x_bytes), rows, n_out,
+          p.ld_terms, p.terms);
       RF_TRY(check_launch("k_grad_terms"));
-      g = ws;
+      g = ws + p.x_bytes;
       ldg = p.ld_terms;
     }
-    CUtensorMap mc, mg;
-    const cuuint64_t cdims[2] = {cuuint64_t(saved->ld), cuuint64_t(rows)}, cstr[1] = {cuuint64_t(saved->ld)};
-    const cuuint32_t cbox[2] = {kHalf, kTokens};
-    RF_TRY(make_map(&mc, CU_TENSOR_MAP_DATA_TYPE_UINT8, saved->codes, 2, cdims, cstr, cbox, CU_TENSOR_MAP_SWIZZLE_NONE));
-    const cuuint64_t gdims[3] = {cuuint64_t(n_out), cuuint64_t(rows), cuuint64_t(p.terms)};
-    const cuuint64_t gstr[2] = {cuuint64_t(ldg) * 2, cuuint64_t(ldg) * 2 * cuuint64_t(rows)};
-    const cuuint32_t gbox[3] = {64, kTokens, 1};
-    RF_TRY(make_map(&mg, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g, 3, gdims, gstr, gbox, CU_TENSOR_MAP_SWIZZLE_128B));
-    Params P{};
-    P.scales = saved->scales;
-    P.scale_rows = saved->scale_rows;
-    P.m = m;
-    P.n = n;
-    P.rows = rows;
-    P.tiles_i = int(ceil_div(m, kTile));
-    P.tiles_j = int(ceil_div(n, kTile));
-    P.splits = p.splits;
-    P.units = int64_t(P.tiles_i) * P.tiles_j * p.splits;
-    P.steps = int(p.steps);
-    P.terms = p.terms;
-    P.x_first = layout == RF_IN_OUT;
-    P.panels = int(ceil_div(features, kPanel8));
-    P.format = saved->format;
-    P.initial = initial;
-    P.out = out;
-    P.ld_out = ld_out;
-    P.out_dt = out_dtype;
-    P.partial = partial;
-    P.ld_partial = p.ld_partial;
-    P.error = device_error_word();
-    // bfloat16 operands, float32 accumulator, both operands MN-major.
-    P.idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | (uint32_t(kTile >> 3) << 17) |
-              (uint32_t(kTile >> 4) << 24);
-    RF_TRY(saved->format == RF_INT8 ? launch<RF_INT8>(mc, mg, P, st) : launch<RF_E4M3>(mc, mg, P, st));
-    if (p.splits == 1) return RF_OK;
+    CUtensorMap mx, mg;
+    RF_TRY(make_map(&mx, ws, features, rows, 1, p.ld_x));
+    RF_TRY(make_map(&mg, g, n_out, rows, p.terms, ldg));
+    RF_TRY(allow_smem());
+    const int64_t pairs = std::min(P.units, max_pairs());
+    k_weight_grad<<<unsigned(2 * pairs), kThreads, kSmemBytes, st>>>(mx, mg, P);
+    RF_TRY(check_launch("k_weight_grad"));
   }
-  const int64_t nv = ceil_div(n, 4);
-  const int tx = int(nv < 256 ? nv : 256), ty = 256 / tx;
-  const int64_t gx = std::min<int64_t>(ceil_div(m, ty), 65535);
-  k_weight_grad_join<<<dim3(unsigned(gx), unsigned(ceil_div(nv, tx))), dim3(unsigned(tx), unsigned(ty)), 0, st>>>(
-      partial, p.splits, m, n, p.ld_partial, initial, out, ld_out, out_dtype);
+  if (P.whole == tiles) return RF_OK;
+  k_weight_grad_join<<<unsigned((tiles - P.whole) * (kTile / 4)), 256, 0, st>>>(P);
   return check_launch("k_weight_grad_join");
 }

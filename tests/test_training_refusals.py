@@ -127,11 +127,14 @@ def test_c_abi_weight_gradient_plans_and_refuses():
         _lib.check(lib.rf_weight_gradient_workspace_size(rows, k, out, ptr, ld, dt, ctypes.byref(n)))
         return n.value
 
-    assert plan(8192, 4096, 14336, 4096, 14336, _lib.RF_BF16) == 0          # a wave of tiles, read in place
-    assert plan(8192, 4096, 14336, 4098, 14336, _lib.RF_BF16) == 8192 * 14336 * 2   # misaligned: copied
-    assert plan(8192, 4096, 14336, 4096, 14336, _lib.RF_F32) == 3 * 8192 * 14336 * 2
+    x, tile = 8192 * 4096 * 2, 256 * 256 * 4
+    whole = plan(8192, 4096, 74 * 256, 4096, 74 * 256, _lib.RF_BF16)           # full waves of tiles, read in place
+    assert whole == x                                                        # the expanded activation
+    assert plan(8192, 4096, 74 * 256, 4098, 74 * 256, _lib.RF_BF16) == x + 8192 * 74 * 256 * 2   # misaligned: copied
+    assert plan(8192, 4096, 74 * 256, 4096, 74 * 256, _lib.RF_F32) == x + 3 * 8192 * 74 * 256 * 2
     assert plan(0, 40, 24, None, 24, _lib.RF_F32) == 0
-    assert plan(4096, 768, 768, 4096, 768, _lib.RF_BF16) % (768 * 768 * 4) == 0      # partial tiles
+    split = plan(4096, 768, 768, 4096, 768, _lib.RF_BF16) - 4096 * 768 * 2
+    assert split > 0 and split % (9 * tile) == 0                             # 9 tiles, each in parts
     _invalid(lib.rf_weight_gradient_workspace_size(4, 40, 24, None, 23, 1, ctypes.byref(n)))
     _invalid(lib.rf_weight_gradient_workspace_size(4, 40, 0, None, 24, 1, ctypes.byref(n)))
     _invalid(lib.rf_weight_gradient_workspace_size(4, 40, 24, None, 24, 9, ctypes.byref(n)))
@@ -142,8 +145,7 @@ def test_c_abi_weight_gradient_plans_and_refuses():
         bad = list(ok)
         bad[i] = v
         _invalid(lib.rf_weight_gradient(*bad))
-    need = list(ok)
-    need[3] = _lib.RF_F32  # terms need a workspace
+    need = list(ok)  # the expanded activation needs a workspace
     _invalid(lib.rf_weight_gradient(*need))
     need[10], need[11] = 4097, 1 << 20
     _invalid(lib.rf_weight_gradient(*need))
