@@ -21,91 +21,10 @@
 // writes one partial row; a second kernel adds the partials in order.
 #include <algorithm>
 
-#include "rf_act8.cuh"
-#include "rf_kernels.cuh"
+#include "rf_block_norm.cuh"
 
 namespace rf {
 namespace bn {
-
-constexpr int64_t kMaxNorm = 16384;
-constexpr int kWarpsPerCta = 4;  // warp-per-row CTAs
-
-struct Param {
-  const void* p;
-  int32_t dt;
-};
-struct Common {
-  int64_t rows, d;
-  int64_t gate_rows;
-  Param pre_w, pre_b, post_w, post_b, scale, gate;
-  float eps, scale_value, inv_d;
-  int32_t post_norm, scale_per_channel, gate_per_channel, gate_act;
-};
-
-struct FwdArgs {
-  Common c;
-  RowView x, b;
-  RowOut x_out, y;
-  Saved8 sx, sb, sy;  // codes null: not saved
-};
-
-struct BwdArgs {
-  Common c;
-  RowView gx, gy;      // gradients of x' and y; p null: absent
-  RowView x, b;
-  Saved8 sx, sb;       // codes set: read instead of x, b
-  RowOut dx, db;
-  void* dgate;         // gate varying by row: written here
-  int32_t row_gate;    // gate varies by row
-  float* partial;      // [items][sums][ldp]
-  int64_t ldp;
-  int64_t items, chunks, rows_per_chunk, group_rows;
-};
-
-// A parameter's 8 values at a column, `absent` where there is none.
-__device__ __forceinline__ void param8(const Param& w, int64_t col, int64_t d, float absent, float (&f)[8]) {
-  if (!w.p) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = absent;
-    return;
-  }
-  const RowView v{w.p, 0, w.dt, (reinterpret_cast<uintptr_t>(w.p) & 15) == 0};
-  load8(v, 0, col, d, f);
-}
-__device__ __forceinline__ float gate_value(float g, int act) {
-  return act == RF_GATE_SIGMOID ? 1.f / (1.f + expf(-g)) : act == RF_GATE_TANH ? tanhf(g) : g;
-}
-// Derivative from the value.
-__device__ __forceinline__ float gate_slope(float a, int act) {
-  return act == RF_GATE_SIGMOID ? a * (1.f - a) : act == RF_GATE_TANH ? 1.f - a * a : 1.f;
-}
-// s a(gamma) at 8 columns of a row, or a alone (times_scale false).
-__device__ __forceinline__ void gate8(const Common& c, int64_t row, int64_t col, float (&f)[8]) {
-  if (!c.gate.p) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = 1.f;
-    return;
-  }
-  const int64_t g = row / c.gate_rows;
-  if (c.gate_per_channel) {
-    load8(row_view_dev(c.gate.p, c.d, c.gate.dt), g, col, c.d, f);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = gate_value(f[k], c.gate_act);
-  } else {
-    const float a = gate_value(ld_as_float(c.gate.p, c.gate.dt, g), c.gate_act);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = a;
-  }
-}
-__device__ __forceinline__ void scale8(const Common& c, int64_t col, float (&f)[8]) {
-  if (c.scale.p && c.scale_per_channel) {
-    param8(c.scale, col, c.d, 1.f, f);
-    return;
-  }
-  const float s = c.scale.p ? ld_as_float(c.scale.p, c.scale.dt, 0) : c.scale_value;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) f[k] = s;
-}
 
 // Sums of N values over a team.  A CTA's sum goes through one of two buffers
 // in turn, so that one barrier per sum is enough; every thread adds the
@@ -552,9 +471,8 @@ Team team_of(int64_t d) {
   return {int(round_up(ceil_div(nv, v), 32)), v, false};
 }
 
-// Rows of an item, and how many items: about three rows of partial sums per
-// SM, never a row of them for fewer than 8 rows of a group unless the group
-// is that short.
+// Rows of an item, and how many items; never a row of partial sums for fewer
+// than 2 rows of a team unless the group is that short.
 struct Split {
   int64_t groups, group_rows, chunks, rows_per_chunk, items;
 };
@@ -563,9 +481,9 @@ Split split_rows(const rf_block_norm& p) {
   const bool grouped = p.gate.value && p.gate_rows > 1;
   s.group_rows = grouped ? p.gate_rows : p.rows;
   s.groups = p.rows == 0 ? 0 : p.rows / s.group_rows;
-  const Team t = team_of(p.features);
-  const int64_t target = 148 * (t.warp ? 8 : 3);
-  const int64_t per = t.warp ? 8 * kWarpsPerCta : 8;
+  // An item for each SM, which holds one CTA of the typed kernels.
+  const int64_t target = 148;
+  const int64_t per = 2 * typed_team(p.features).teams;
   if (s.groups > 0) {
     const int64_t want = std::max<int64_t>(1, target / s.groups);
     s.chunks = std::max<int64_t>(1, std::min(want, s.group_rows / per));
@@ -748,6 +666,7 @@ extern "C" rf_status rf_block_norm_forward(const rf_block_norm* p, const rf_rows
   if (saved_y) A.sy = saved8(*saved_y);
   const Team t = team_of(d);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (try_typed_fwd(*p, A, st)) return check_launch("k_norm_fwd_typed");
   if (p->kind == RF_LAYER_NORM) launch_fwd<true>(t, A, st);
   else launch_fwd<false>(t, A, st);
   return check_launch("k_norm_fwd");
@@ -808,12 +727,14 @@ extern "C" rf_status rf_block_norm_backward(const rf_block_norm* p, const rf_row
     A.dgate = A.row_gate ? p->gate.grad : nullptr;
     A.partial = n.cols ? partial : nullptr;
     A.ldp = ldp;
+    A.sums = n.bias ? 4 : 2;
     A.items = s.items;
     A.chunks = s.chunks;
     A.rows_per_chunk = s.rows_per_chunk;
     A.group_rows = s.group_rows;
     const Team t = team_of(d);
-    if (p->kind == RF_LAYER_NORM) n.bias ? launch_bwd<true, true>(t, A, st) : launch_bwd<true, false>(t, A, st);
+    if (try_typed_bwd(*p, A, n.bias, st)) {
+    } else if (p->kind == RF_LAYER_NORM) n.bias ? launch_bwd<true, true>(t, A, st) : launch_bwd<true, false>(t, A, st);
     else n.bias ? launch_bwd<false, true>(t, A, st) : launch_bwd<false, false>(t, A, st);
     RF_TRY(check_launch("k_norm_bwd"));
   }
