@@ -164,23 +164,6 @@ __device__ __forceinline__ uint2 encode8_stochastic(const float (&f)[8], uint64_
   return format == RF_INT8 ? encode8_stochastic_int8(f, a, b, s) : encode8_stochastic_e4m3(f, a, b, s);
 }
 
-// Step byte of a block straight from 16-bit elements: their magnitudes' bits
-// order like the magnitudes, two at a time.
-template <int DT>
-__device__ __forceinline__ uint32_t raw_max_bits(const Raw8<DT>& r) {
-  if (DT == RF_F32) {
-    float f[8];
-    unpack<DT>(r, f);
-    return block_max_bits(f);
-  }
-  uint32_t m = __vmaxu2(__vmaxu2(r.u[0].x & 0x7FFF7FFFu, r.u[0].y & 0x7FFF7FFFu),
-                        __vmaxu2(r.u[0].z & 0x7FFF7FFFu, r.u[0].w & 0x7FFF7FFFu));
-  m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-  m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-  m = max(m & 0xFFFFu, m >> 16);
-  return DT == RF_BF16 ? m << 16 : __float_as_uint(__half2float(__ushort_as_half(uint16_t(m))));
-}
-
 // One thread's column of an array, walked down by rows.  Addresses move by
 // constant strides: as products of 64-bit row numbers they were a third of
 // the save kernel's instructions.

@@ -258,6 +258,23 @@ __device__ __forceinline__ uint32_t block_max_bits(const float (&f)[8]) {
   return max(a, __shfl_xor_sync(0xFFFFFFFFu, a, 2));
 }
 
+// The same straight from memory's form: the magnitudes' bits of 16-bit types
+// order like the magnitudes too, two at a time.
+template <int DT>
+__device__ __forceinline__ uint32_t raw_max_bits(const Raw8<DT>& r) {
+  if (DT == RF_F32) {
+    float f[8];
+    unpack<DT>(r, f);
+    return block_max_bits(f);
+  }
+  uint32_t m = __vmaxu2(__vmaxu2(r.u[0].x & 0x7FFF7FFFu, r.u[0].y & 0x7FFF7FFFu),
+                        __vmaxu2(r.u[0].z & 0x7FFF7FFFu, r.u[0].w & 0x7FFF7FFFu));
+  m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+  m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+  m = max(m & 0xFFFFu, m >> 16);
+  return DT == RF_BF16 ? m << 16 : __float_as_uint(__half2float(__ushort_as_half(uint16_t(m))));
+}
+
 // 8 values -> 8 codes under step byte s, to nearest even.
 __device__ __forceinline__ uint2 encode8(const float (&f)[8], uint32_t s, int format) {
   if (s == kNanStep) return make_uint2(0u, 0u);

@@ -80,74 +80,146 @@ __device__ __forceinline__ void store_part(const RowOut& t, int64_t i, int n, co
 }
 
 // -- teams ---------------------------------------------------------------------
+// Sums over a row cost more instructions than the row's own arithmetic when
+// every value takes its own five shuffles and every thread adds every warp's
+// part (99 instructions an element, backward).  So values share shuffles: of
+// N = 2 or 4, a lane hands on one half and keeps the other until a half or a
+// quarter of the warp carries each; the warps' parts are added the same way.
 struct TeamSums {
-  float v[2][3][kMaxTeams][kTypedThreads / 32];
+  float v[2][kMaxTeams][4 * 16];  // per buffer and team: N x 16 warps, zeros for warps that are not there
 };
 struct TeamCtx {
-  int lane, threads, warps, id;
+  int lane, threads, id;
+  bool alone;  // one warp
 };
-__device__ __forceinline__ TeamCtx team_ctx(int threads) {
+__device__ __forceinline__ TeamCtx team_ctx(int threads, TeamSums& s) {
   TeamCtx t;
   t.threads = threads;
   t.id = int(threadIdx.x) / threads;
   t.lane = int(threadIdx.x) - t.id * threads;
-  t.warps = threads >> 5;
+  t.alone = threads == 32;
+  for (int i = int(threadIdx.x); i < int(sizeof(s.v) / 4); i += int(blockDim.x)) (&s.v[0][0][0])[i] = 0.f;
+  __syncthreads();
   return t;
 }
+__device__ __forceinline__ float other(float x, int bit) { return __shfl_xor_sync(0xFFFFFFFFu, x, bit); }
+// Two values into one: lanes with `bit` go on with b, the others with a.
+__device__ __forceinline__ float fold(float a, float b, int lane, int bit) {
+  const bool hi = lane & bit;
+  return (hi ? b : a) + other(hi ? a : b, bit);
+}
 // Sums of N values over a team, through one of two buffers in turn, so that
-// one barrier per sum is enough: the team's own (0 is the CTA's).  Every
-// thread adds the warps' values in the same order.
+// one barrier per sum is enough: the team's own (0 is the CTA's).  All threads
+// get the same bits.
 template <int N>
 __device__ __forceinline__ void sum_over(float (&v)[N], const TeamCtx& t, TeamSums& s, int& turn) {
+  static_assert(N == 1 || N == 2 || N == 4, "");
+  constexpr int kSpan = 32 / N;  // lanes that carry one value
+  const int lane = t.lane & 31;
+  float x;
+  if (N == 1) x = v[0] + other(v[0], 16);
+  else if (N == 2) x = fold(v[0], v[N - 1], lane, 16);
+  else x = fold(fold(v[0], v[N == 4 ? 2 : 0], lane, 16), fold(v[N == 4 ? 1 : 0], v[N - 1], lane, 16), lane, 8);
 #pragma unroll
-  for (int o = 16; o; o >>= 1)
+  for (int o = N == 1 ? 8 : kSpan / 2; o; o >>= 1) x += other(x, o);
+  if (!t.alone) {
+    float* part = s.v[turn][t.id];
+    if ((lane & (kSpan - 1)) == 0) part[(lane / kSpan) * 16 + (t.lane >> 5)] = x;
+    asm volatile("bar.sync %0, %1;" ::"r"(t.id + 1), "r"(t.threads) : "memory");
+    if (N == 4) {
+      const float2 p = *reinterpret_cast<const float2*>(part + (lane >> 3) * 16 + (lane & 7) * 2);
+      x = p.x + p.y;
+    } else {
+      x = part[N == 2 ? lane : lane & 15];
+    }
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xFFFFFFFFu, v[i], o);
-  if (t.warps == 1) return;
-  if ((t.lane & 31) == 0)
-#pragma unroll
-    for (int i = 0; i < N; ++i) s.v[turn][i][t.id][t.lane >> 5] = v[i];
-  asm volatile("bar.sync %0, %1;" ::"r"(t.id + 1), "r"(t.threads) : "memory");
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float x = 0.f;
-    for (int w = 0; w < t.warps; ++w) x += s.v[turn][i][t.id][w];
-    v[i] = x;
+    for (int o = N == 4 ? 4 : 8; o; o >>= 1) x += other(x, o);
+    turn ^= 1;
   }
-  turn ^= 1;
+  if (N == 1) v[0] = x;
+  else
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xFFFFFFFFu, x, i * kSpan);
 }
-// Normalises a row in place and returns its factor; places behind the last
-// feature (n[v] of a vector are before it) hold 0 and stay 0.  The variance is
-// taken around the mean, a second pass over the registers, so a large mean
-// costs no digits.
-template <int V, bool kLayer>
-__device__ __forceinline__ float normalise_row(float (&f)[V][8], const int (&n)[V], const Common& c, const TeamCtx& t,
-                                               TeamSums& s, int& turn) {
-  if (kLayer) {
-    float m[1] = {0.f};
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) m[0] += f[v][k];
-    sum_over(m, t, s, turn);
-    const float mean = m[0] * c.inv_d;
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[v][k] = k < n[v] ? f[v][k] - mean : 0.f;
-  }
-  float q[1] = {0.f};
+
+template <int V>
+__device__ __forceinline__ float sum8(const float (&f)[V][8]) {
+  float s = 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) q[0] = fmaf(f[v][k], f[v][k], q[0]);
-  sum_over(q, t, s, turn);
-  const float r = rsqrtf(fmaf(q[0], c.inv_d, c.eps));
+    for (int k = 0; k < 8; ++k) s += f[v][k];
+  return s;
+}
+template <int V>
+__device__ __forceinline__ float dot8(const float (&f)[V][8], const float (&g)[V][8]) {
+  float s = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s = fmaf(f[v][k], g[v][k], s);
+  return s;
+}
+// Takes a mean off; places behind the last feature (n[v] of a vector are
+// before it) stay 0.
+template <int V>
+__device__ __forceinline__ void centre(float (&f)[V][8], float mean, const int (&n)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[v][k] = k < n[v] ? f[v][k] - mean : 0.f;
+}
+template <int V>
+__device__ __forceinline__ void times(float (&f)[V][8], float r) {
 #pragma unroll
   for (int v = 0; v < V; ++v)
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[v][k] *= r;
-  return r;
+}
+__device__ __forceinline__ float factor(float sum_sq, const Common& c) { return rsqrtf(fmaf(sum_sq, c.inv_d, c.eps)); }
+// Normalises a row in place.  The variance is taken around the mean, a second
+// pass over the registers, so a large mean costs no digits.
+template <int V, bool kLayer>
+__device__ __forceinline__ void normalise_row(float (&f)[V][8], const int (&n)[V], const Common& c, const TeamCtx& t,
+                                              TeamSums& s, int& turn) {
+  if (kLayer) {
+    float m[1] = {sum8<V>(f)};
+    sum_over(m, t, s, turn);
+    centre<V>(f, m[0] * c.inv_d, n);
+  }
+  float q[1] = {dot8<V>(f, f)};
+  sum_over(q, t, s, turn);
+  times<V>(f, factor(q[0], c));
+}
+// Element offset of a row's column; strides here are below 2^31.
+__device__ __forceinline__ int64_t at(int row, int64_t ld, int col) {
+  return int64_t(uint64_t(uint32_t(row)) * uint32_t(ld) + uint32_t(col));
+}
+// A thread's place in a saved activation, without the row.
+struct SavedPlace {
+  int64_t step0;
+  bool codes, step;
+};
+__device__ __forceinline__ SavedPlace saved_place(const Saved8& s, int col, int64_t d) {
+  SavedPlace p;
+  const bool in = s.codes && col < (int(d) + kPanel8 - 1) / kPanel8 * kPanel8;
+  p.codes = in && col < s.ld;
+  p.step = in && (col & (kBlock8 - 1)) == 0;
+  p.step0 = in ? scale_index(s, 0, col) : 0;
+  return p;
+}
+template <int DT>
+__device__ __forceinline__ uint32_t raw_step(const Raw8<DT>& r, int format) {
+  return step_byte(raw_max_bits<DT>(r), format);
+}
+// A vector as it lies in memory (raw, f its values) into a saved row.
+template <int DT>
+__device__ __forceinline__ void save_raw(const Saved8& s, const SavedPlace& p, int row, int col, const Raw8<DT>& raw,
+                                         const float (&f)[8]) {
+  const uint32_t st = raw_step<DT>(raw, s.format);
+  const uint2 c = encode8(f, st, s.format);
+  if (p.codes) *reinterpret_cast<uint2*>(s.codes + at(row, s.ld, col)) = c;
+  if (p.step) s.scales[p.step0 + 4 * int64_t(row)] = uint8_t(st);
 }
 template <int V>
 __device__ __forceinline__ void own_columns(const TeamCtx& t, const Common& c, int (&col)[V], int (&n)[V]) {
@@ -166,16 +238,20 @@ __global__ void __launch_bounds__(kTypedThreads, V == 1 ? 2 : 1)
   __shared__ TeamSums sums;
   int turn = 0;
   const Common& c = A.c;
-  const TeamCtx t = team_ctx(team_threads);
+  const TeamCtx t = team_ctx(team_threads, sums);
   const int teams = int(blockDim.x) / team_threads;
   const int64_t step = int64_t(gridDim.x) * teams;
   const bool has_b = A.b.p != nullptr, has_y = A.y.p != nullptr, fixed = gate_is_fixed(c);
   // x' = x + normalised * mul + add;  y = normalised * pw + pb
   float mul[V][8], pw[V][8], add[kLayer ? V : 1][8], pb[kLayer ? V : 1][8];
   int col[V], n[V];
+  SavedPlace px[V], pbr[V], py[V];
   own_columns<V>(t, c, col, n);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
+    px[v] = saved_place(A.sx, col[v], c.d);
+    pbr[v] = saved_place(A.sb, col[v], c.d);
+    py[v] = saved_place(A.sy, col[v], c.d);
     float w[8], g[8];
     param8(c.pre_w, col[v], c.d, 1.f, pw[v]);
     scale8(c, col[v], w);
@@ -194,54 +270,64 @@ __global__ void __launch_bounds__(kTypedThreads, V == 1 ? 2 : 1)
       for (int k = 0; k < 8; ++k) add[v][k] = k < n[v] ? g[k] * w[k] : 0.f;
     }
   }
-  int64_t row = int64_t(blockIdx.x) * teams + t.id;
+  const int rows = int(c.rows);
+  int64_t next = int64_t(blockIdx.x) * teams + t.id;  // up to 2^31 and a step beyond
   Raw8<XT> nx[V];
   Raw8<BT> nb[V];
-  auto fetch = [&](int64_t at) {
+  auto fetch = [&]() {
+    const bool live = next < rows;
+    const int r = live ? int(next) : 0;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      nx[v] = load_part<XT>(A.x, at * A.x.ld + col[v], at < c.rows ? n[v] : 0);
-      nb[v] = load_part<BT>(A.b, at * A.b.ld + col[v], at < c.rows && has_b ? n[v] : 0);
+      nx[v] = load_part<XT>(A.x, at(r, A.x.ld, col[v]), live ? n[v] : 0);
+      nb[v] = load_part<BT>(A.b, at(r, A.b.ld, col[v]), live && has_b ? n[v] : 0);
     }
   };
-  fetch(row);
-  for (; row < c.rows; row += step) {
+  fetch();
+  while (next < rows) {
+    const int row = int(next);
+    Raw8<XT> rx[V];
+    Raw8<BT> rb[V];
     float x[V][8], b[V][8];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      unpack<XT>(nx[v], x[v]);
-      unpack<BT>(nb[v], b[v]);
+      rx[v] = nx[v];
+      rb[v] = nb[v];
+      unpack<XT>(rx[v], x[v]);
+      unpack<BT>(rb[v], b[v]);
     }
-    fetch(row + step);
+    next += step;
+    fetch();
     if (has_b) {
       if (A.sb.codes) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) save_row8(A.sb, row, col[v], c.d, b[v]);
+        for (int v = 0; v < V; ++v) save_raw<BT>(A.sb, pbr[v], row, col[v], rb[v], b[v]);
       }
       if (c.post_norm) normalise_row<V, kLayer>(b, n, c, t, sums, turn);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
+        if (fixed) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) b[v][k] = kLayer ? fmaf(b[v][k], mul[v][k], add[kLayer ? v : 0][k]) : b[v][k] * mul[v][k];
-        if (!fixed) {
+          for (int k = 0; k < 8; ++k)
+            x[v][k] = fmaf(b[v][k], mul[v][k], kLayer ? x[v][k] + add[kLayer ? v : 0][k] : x[v][k]);
+        } else {
           float g[8];
           gate8(c, row, col[v], g);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) b[v][k] *= g[k];
+          for (int k = 0; k < 8; ++k)
+            x[v][k] = fmaf(kLayer ? fmaf(b[v][k], mul[v][k], add[kLayer ? v : 0][k]) : b[v][k] * mul[v][k], g[k], x[v][k]);
         }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[v][k] += b[v][k];
-        const Raw8<XT> raw = pack<XT>(x[v]);
-        if (n[v]) store_part<XT>(A.x_out, row * A.x_out.ld + col[v], n[v], raw);
-        if (A.sx.codes) {
-          float r[8];
-          unpack<XT>(raw, r);
-          save_row8(A.sx, row, col[v], c.d, r);
-        }
+        rx[v] = pack<XT>(x[v]);
+        if (n[v]) store_part<XT>(A.x_out, at(row, A.x_out.ld, col[v]), n[v], rx[v]);
       }
-    } else if (A.sx.codes) {
+    }
+    if (A.sx.codes) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) save_row8(A.sx, row, col[v], c.d, x[v]);
+      for (int v = 0; v < V; ++v) {
+        float f[8];
+        unpack<XT>(rx[v], f);
+        save_raw<XT>(A.sx, px[v], row, col[v], rx[v], f);
+      }
     }
     if (!has_y) continue;
     normalise_row<V, kLayer>(x, n, c, t, sums, turn);
@@ -250,10 +336,10 @@ __global__ void __launch_bounds__(kTypedThreads, V == 1 ? 2 : 1)
 #pragma unroll
       for (int k = 0; k < 8; ++k) x[v][k] = kLayer ? fmaf(x[v][k], pw[v][k], pb[kLayer ? v : 0][k]) : x[v][k] * pw[v][k];
       const Raw8<BT> raw = pack<BT>(x[v]);
-      if (n[v]) store_part<BT>(A.y, row * A.y.ld + col[v], n[v], raw);
+      if (n[v]) store_part<BT>(A.y, at(row, A.y.ld, col[v]), n[v], raw);
       if (A.sy.codes) {
         unpack<BT>(raw, x[v]);
-        save_row8(A.sy, row, col[v], c.d, x[v]);
+        save_raw<BT>(A.sy, py[v], row, col[v], raw, x[v]);
       }
     }
   }
@@ -263,8 +349,8 @@ __global__ void __launch_bounds__(kTypedThreads, V == 1 ? 2 : 1)
 template <int DT, bool kSaved>
 struct Held {
   Raw8<DT> raw;
-  __device__ __forceinline__ void fetch(const RowView& t, const Saved8&, int64_t row, int64_t col, int n) {
-    raw = load_part<DT>(t, row * t.ld + col, n);
+  __device__ __forceinline__ void fetch(const RowView& t, const Saved8&, int64_t, int row, int col, int n) {
+    raw = load_part<DT>(t, at(row, t.ld, col), n);
   }
   __device__ __forceinline__ void values(const Saved8&, float (&f)[8]) const { unpack<DT>(raw, f); }
 };
@@ -272,11 +358,10 @@ template <int DT>
 struct Held<DT, true> {
   uint2 codes;
   uint32_t step;
-  __device__ __forceinline__ void fetch(const RowView&, const Saved8& s, int64_t row, int64_t col, int n) {
-    codes = n ? __ldg(reinterpret_cast<const uint2*>(s.codes + row * s.ld + col)) : make_uint2(0, 0);
-    step = n ? __ldg(s.scales + scale_index(s, row, col)) : 1u;
+  __device__ __forceinline__ void fetch(const RowView&, const Saved8& s, int64_t step0, int row, int col, int n) {
+    codes = n ? __ldg(reinterpret_cast<const uint2*>(s.codes + at(row, s.ld, col))) : make_uint2(0, 0);
+    step = n ? __ldg(s.scales + step0 + 4 * int64_t(row)) : 1u;
   }
-  // Codes behind the last feature are 0; a NaN step must not reach them.
   __device__ __forceinline__ void values(const Saved8& s, float (&f)[8]) const {
     decode4(codes.x, s.format, f);
     decode4(codes.y, s.format, f + 4);
@@ -294,20 +379,25 @@ __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __gri
   extern __shared__ float join[];        // [kSums][team_threads * 8 V] when a CTA has several teams
   int turn = 0;
   const Common& c = A.c;
-  const TeamCtx t = team_ctx(team_threads);
+  const TeamCtx t = team_ctx(team_threads, sums);
   const int teams = int(blockDim.x) / team_threads;
   const bool has_y = A.gy.p != nullptr, has_gx = A.gx.p != nullptr;
   const bool has_b = A.b.p != nullptr || A.sb.codes != nullptr;
+  const bool token_gate = A.row_gate && A.dgate && !c.gate_per_channel;
   float pw[V][8];
   int col[V], n[V];
+  int64_t step0[V];  // x and b are saved alike, so their steps lie at the same offsets
   own_columns<V>(t, c, col, n);
 #pragma unroll
-  for (int v = 0; v < V; ++v) param8(c.pre_w, col[v], c.d, 1.f, pw[v]);
+  for (int v = 0; v < V; ++v) {
+    param8(c.pre_w, col[v], c.d, 1.f, pw[v]);
+    step0[v] = kSaved && n[v] ? scale_index(A.sx.codes ? A.sx : A.sb, 0, col[v]) : 0;
+  }
 
   for (int64_t item = blockIdx.x; item < A.items; item += gridDim.x) {
     const int64_t group = item / A.chunks;
-    const int64_t first = group * A.group_rows + (item - group * A.chunks) * A.rows_per_chunk;
-    const int64_t last = min(first + A.rows_per_chunk, (group + 1) * A.group_rows);
+    const int64_t first64 = group * A.group_rows + (item - group * A.chunks) * A.rows_per_chunk;
+    const int first = int(first64), last = int(min(first64 + A.rows_per_chunk, (group + 1) * A.group_rows));
     // h = e mul: the scale, w_post, and the group's gate unless it varies by row.
     float mul[V][8];
 #pragma unroll
@@ -335,61 +425,76 @@ __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __gri
     Raw8<BT> ngy[V];
     Held<XT, kSaved> nx[V];
     Held<BT, kSaved> nb[V];
-    auto fetch = [&](int64_t at) {
+    auto fetch = [&](int r) {
+      const bool in = r < last && r >= 0;  // r may pass 2^31 behind the last row
+      const int row = in ? r : first;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const int live = at < last ? n[v] : 0;
-        ngx[v] = load_part<XT>(A.gx, at * A.gx.ld + col[v], has_gx ? live : 0);
-        ngy[v] = load_part<BT>(A.gy, at * A.gy.ld + col[v], has_y ? live : 0);
-        nx[v].fetch(A.x, A.sx, at, col[v], has_y ? live : 0);
-        nb[v].fetch(A.b, A.sb, at, col[v], has_b ? live : 0);
+        const int live = in ? n[v] : 0;
+        ngx[v] = load_part<XT>(A.gx, at(row, A.gx.ld, col[v]), has_gx ? live : 0);
+        ngy[v] = load_part<BT>(A.gy, at(row, A.gy.ld, col[v]), has_y ? live : 0);
+        nx[v].fetch(A.x, A.sx, step0[v], row, col[v], has_y ? live : 0);
+        nb[v].fetch(A.b, A.sb, step0[v], row, col[v], has_b ? live : 0);
       }
     };
     if (kAhead) fetch(first + t.id);
-    for (int64_t row = first + t.id; row < last; row += teams) {
+    for (int64_t row64 = first + t.id; row64 < last; row64 += teams) {
+      const int row = int(row64);
       if (!kAhead) fetch(row);
-      float e[V][8], b[V][8];
+      float e[V][8], b[V][8], x[V][8], g[V][8];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        unpack<XT>(ngx[v], e[v]);
+        unpack<BT>(ngy[v], g[v]);
+        nx[v].values(A.sx, x[v]);
+        nb[v].values(A.sb, b[v]);
+      }
+      if (kAhead) fetch(int(uint32_t(row) + uint32_t(teams)));
+
+      // Row sums.  RMS in one round, of the raw x: with n = r x, sum g n is
+      // r sum g x.  LayerNorm takes the means off first.
+      float sxx, sgx, sg = 0.f, sbb;
+      if (kLayer) {
+        float m[2] = {sum8<V>(x), sum8<V>(b)};
+        sum_over(m, t, sums, turn);
+        centre<V>(x, m[0] * c.inv_d, n);
+        if (c.post_norm) centre<V>(b, m[1] * c.inv_d, n);
+      }
       {
-        float x[V][8], g[V][8];
+        float gw[V][8];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          unpack<XT>(ngx[v], e[v]);
-          unpack<BT>(ngy[v], g[v]);
-          nx[v].values(A.sx, x[v]);
-          nb[v].values(A.sb, b[v]);
-        }
-        if (kAhead) fetch(row + teams);
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) gw[v][k] = g[v][k] * pw[v][k];
+        float s[4] = {dot8<V>(x, x), dot8<V>(gw, x), dot8<V>(b, b), kLayer ? sum8<V>(gw) : 0.f};
+        sum_over(s, t, sums, turn);
+        sxx = s[0];
+        sgx = s[1];
+        sbb = s[2];
+        sg = s[3];
         if (has_y) {
-          const float r = normalise_row<V, kLayer>(x, n, c, t, sums, turn);
-          float s[2] = {0.f, 0.f};
+          const float r = factor(sxx, c);
+          const float mgn = sgx * r * c.inv_d, mg = kLayer ? sg * c.inv_d : 0.f;
 #pragma unroll
           for (int v = 0; v < V; ++v)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              acc[1][v][k] = fmaf(g[v][k], x[v][k], acc[1][v][k]);
+              const float nk = x[v][k] * r;
+              acc[1][v][k] = fmaf(g[v][k], nk, acc[1][v][k]);
               if (kLayer) acc[kSums - 1][v][k] += g[v][k];
-              g[v][k] *= pw[v][k];
-              s[0] = fmaf(g[v][k], x[v][k], s[0]);
-              if (kLayer) s[1] += g[v][k];
-            }
-          sum_over(s, t, sums, turn);
-          const float mgn = s[0] * c.inv_d, mg = kLayer ? s[1] * c.inv_d : 0.f;
-#pragma unroll
-          for (int v = 0; v < V; ++v)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              e[v][k] = fmaf(r, fmaf(-x[v][k], mgn, kLayer ? g[v][k] - mg : g[v][k]), e[v][k]);
+              e[v][k] = fmaf(r, fmaf(-nk, mgn, kLayer ? gw[v][k] - mg : gw[v][k]), e[v][k]);
               if (kLayer && k >= n[v]) e[v][k] = 0.f;
             }
         }
       }
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (n[v]) store_part<XT>(A.dx, row * A.dx.ld + col[v], n[v], pack<XT>(e[v]));
+        if (n[v]) store_part<XT>(A.dx, at(row, A.dx.ld, col[v]), n[v], pack<XT>(e[v]));
       if (!has_b) continue;
 
-      const float rb = c.post_norm ? normalise_row<V, kLayer>(b, n, c, t, sums, turn) : 1.f;
-      float s[3] = {0.f, 0.f, 0.f};  // sum h m, sum h, sum e s n (a gate per row)
+      const float rb = c.post_norm ? factor(sbb, c) : 1.f;
+      times<V>(b, rb);
+      float token = 0.f;  // sum e s n, the gradient of a gate per row
       if (A.row_gate) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -408,8 +513,16 @@ __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __gri
           }
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            s[2] += f[k];
+            token += f[k];
             e[v][k] *= a[k];
+          }
+        }
+        if (token_gate) {
+          float s[1] = {token};
+          sum_over(s, t, sums, turn);
+          if (t.lane == 0) {
+            const float a = gate_value(ld_as_float(c.gate.p, c.gate.dt, row), c.gate_act);
+            st_from_float(A.dgate, c.gate.dt, row, s[0] * gate_slope(a, c.gate_act));
           }
         }
       }
@@ -420,19 +533,19 @@ __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __gri
           acc[0][v][k] = fmaf(e[v][k], b[v][k], acc[0][v][k]);
           if (kLayer) acc[kLayer ? 2 : 0][v][k] += e[v][k];
           e[v][k] *= mul[v][k];
-          s[0] = fmaf(e[v][k], b[v][k], s[0]);
-          if (kLayer) s[1] += e[v][k];
         }
-      const bool token_gate = A.row_gate && A.dgate && !c.gate_per_channel;
-      if (c.post_norm || token_gate) {
-        sum_over(s, t, sums, turn);
-        if (token_gate && t.lane == 0) {
-          const float a = gate_value(ld_as_float(c.gate.p, c.gate.dt, row), c.gate_act);
-          st_from_float(A.dgate, c.gate.dt, row, s[2] * gate_slope(a, c.gate_act));
-        }
-      }
       if (c.post_norm) {
-        const float mhm = s[0] * c.inv_d, mh = kLayer ? s[1] * c.inv_d : 0.f;
+        float mhm, mh = 0.f;
+        if (kLayer) {
+          float s[2] = {dot8<V>(e, b), sum8<V>(e)};
+          sum_over(s, t, sums, turn);
+          mhm = s[0] * c.inv_d;
+          mh = s[1] * c.inv_d;
+        } else {
+          float s[1] = {dot8<V>(e, b)};
+          sum_over(s, t, sums, turn);
+          mhm = s[0] * c.inv_d;
+        }
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
@@ -440,7 +553,7 @@ __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __gri
       }
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (n[v]) store_part<BT>(A.db, row * A.db.ld + col[v], n[v], pack<BT>(e[v]));
+        if (n[v]) store_part<BT>(A.db, at(row, A.db.ld, col[v]), n[v], pack<BT>(e[v]));
     }
 
     if (!A.partial) continue;
@@ -488,8 +601,9 @@ __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __gri
   }
 }
 
-bool type_is(const RowView& t, int dt) { return !t.p || t.dt == dt; }
-bool type_is(const RowOut& t, int dt) { return !t.p || t.dt == dt; }
+// An absent array, or one of this type with a stride that fits 32 bits.
+bool type_is(const RowView& t, int dt) { return !t.p || (t.dt == dt && t.ld <= 0x7FFFFFFF); }
+bool type_is(const RowOut& t, int dt) { return !t.p || (t.dt == dt && t.ld <= 0x7FFFFFFF); }
 
 // Calls f with the pair of types and V as constants; false for another pair.
 template <typename F>
@@ -521,7 +635,7 @@ TypedTeam typed_team(int64_t d) {
 bool try_typed_fwd(const rf_block_norm& p, const FwdArgs& A, cudaStream_t st) {
   const bool layer = p.kind == RF_LAYER_NORM;
   const int xt = A.x.dt, bt = A.b.p ? A.b.dt : A.y.p ? A.y.dt : xt;
-  if (p.features > kMaxTyped || !type_is(A.x_out, xt) || !type_is(A.y, bt) ||
+  if (p.features > kMaxTyped || !type_is(A.x, xt) || !type_is(A.b, bt) || !type_is(A.x_out, xt) || !type_is(A.y, bt) ||
       (!layer && (p.pre_bias.value || p.post_bias.value)))
     return false;
   const TypedTeam t = typed_team(p.features);
