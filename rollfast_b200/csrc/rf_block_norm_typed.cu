@@ -23,11 +23,14 @@ namespace {
 constexpr int kTypedThreads = 512;
 constexpr int kMaxTeams = 8;
 constexpr int64_t kMaxTyped = 2 * kTypedThreads * 8;
+constexpr int kFwdVectors = 2;  // vectors per thread, forward
 
 // -- vectors of 8, whole or in part --------------------------------------------
-// The first n of 8 elements at i; zeros behind.
-template <int DT>
+// The first n of 8 elements at i; zeros behind.  kVec: rows of whole vectors
+// on 16-byte boundaries, n is 0 or 8.
+template <int DT, bool kVec>
 __device__ __forceinline__ Raw8<DT> load_part(const RowView& t, int64_t i, int n) {
+  if (kVec) return n ? load_raw<DT>(t.p, i) : zero_raw<DT>();
   if (n == 8 && t.vec) return load_raw<DT>(t.p, i);
   Raw8<DT> r = zero_raw<DT>();
   uint32_t w[8];
@@ -61,14 +64,15 @@ __device__ __forceinline__ Raw8<DT> pack(const float (&f)[8]) {
   }
   return r;
 }
-template <int DT>
+template <int DT, bool kVec>
 __device__ __forceinline__ void store_part(const RowOut& t, int64_t i, int n, const Raw8<DT>& r) {
-  if (n == 8 && t.vec) {
+  if (kVec || (n == 8 && t.vec)) {
     uint4* p = reinterpret_cast<uint4*>(static_cast<uint8_t*>(t.p) + i * (DT == RF_F32 ? 4 : 2));
     p[0] = r.u[0];
     if (DT == RF_F32) p[1] = r.u[DT == RF_F32 ? 1 : 0];
-    return;
+    if (kVec) return;
   }
+  if (n == 8 && t.vec) return;
   const uint4 b = r.u[DT == RF_F32 ? 1 : 0];
   const uint32_t w[8] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w, b.x, b.y, b.z, b.w};
 #pragma unroll
@@ -195,32 +199,6 @@ __device__ __forceinline__ void normalise_row(float (&f)[V][8], const int (&n)[V
 __device__ __forceinline__ int64_t at(int row, int64_t ld, int col) {
   return int64_t(uint64_t(uint32_t(row)) * uint32_t(ld) + uint32_t(col));
 }
-// A thread's place in a saved activation, without the row.
-struct SavedPlace {
-  int64_t step0;
-  bool codes, step;
-};
-__device__ __forceinline__ SavedPlace saved_place(const Saved8& s, int col, int64_t d) {
-  SavedPlace p;
-  const bool in = s.codes && col < (int(d) + kPanel8 - 1) / kPanel8 * kPanel8;
-  p.codes = in && col < s.ld;
-  p.step = in && (col & (kBlock8 - 1)) == 0;
-  p.step0 = in ? scale_index(s, 0, col) : 0;
-  return p;
-}
-template <int DT>
-__device__ __forceinline__ uint32_t raw_step(const Raw8<DT>& r, int format) {
-  return step_byte(raw_max_bits<DT>(r), format);
-}
-// A vector as it lies in memory (raw, f its values) into a saved row.
-template <int DT>
-__device__ __forceinline__ void save_raw(const Saved8& s, const SavedPlace& p, int row, int col, const Raw8<DT>& raw,
-                                         const float (&f)[8]) {
-  const uint32_t st = raw_step<DT>(raw, s.format);
-  const uint2 c = encode8(f, st, s.format);
-  if (p.codes) *reinterpret_cast<uint2*>(s.codes + at(row, s.ld, col)) = c;
-  if (p.step) s.scales[p.step0 + 4 * int64_t(row)] = uint8_t(st);
-}
 template <int V>
 __device__ __forceinline__ void own_columns(const TeamCtx& t, const Common& c, int (&col)[V], int (&n)[V]) {
 #pragma unroll
@@ -231,10 +209,27 @@ __device__ __forceinline__ void own_columns(const TeamCtx& t, const Common& c, i
 }
 // A gate that is the same for all rows is part of a column's factor.
 __device__ __forceinline__ bool gate_is_fixed(const Common& c) { return !c.gate.p || c.gate_rows >= c.rows; }
+// Offset of a column's step byte in row 0 of any activation saved with these
+// rows, and whether the column lies in its panels.
+__device__ __forceinline__ int64_t first_step(const Common& c, int col) {
+  const int64_t scale_rows = (c.rows + 63) / 64 * 64;
+  return ((int64_t(col) / kPanel8) * scale_rows) * 4 + (col % kPanel8) / kBlock8;
+}
+// A vector as it lies in memory (raw, f its values) into a saved row.
+template <int DT>
+__device__ __forceinline__ void save_raw(const Saved8& s, const Common& c, int64_t step0, int row, int col,
+                                         const Raw8<DT>& raw, const float (&f)[8]) {
+  const uint32_t st = step_byte(raw_max_bits<DT>(raw), s.format);
+  const uint2 code = encode8(f, st, s.format);
+  if (col < int(s.ld)) *reinterpret_cast<uint2*>(s.codes + at(row, s.ld, col)) = code;
+  if ((col & (kBlock8 - 1)) == 0 && col < (int(c.d) + kPanel8 - 1) / kPanel8 * kPanel8)
+    s.scales[step0 + 4 * int64_t(row)] = uint8_t(st);
+}
 
-template <int XT, int BT, int V, bool kLayer>
-__global__ void __launch_bounds__(kTypedThreads, V == 1 ? 2 : 1)
+template <int XT, int BT, bool kLayer, bool kSave, bool kVec>
+__global__ void __launch_bounds__(kTypedThreads, 1)
     k_norm_fwd_typed(const __grid_constant__ FwdArgs A, int team_threads) {
+  constexpr int V = kFwdVectors;
   __shared__ TeamSums sums;
   int turn = 0;
   const Common& c = A.c;
@@ -245,13 +240,11 @@ __global__ void __launch_bounds__(kTypedThreads, V == 1 ? 2 : 1)
   // x' = x + normalised * mul + add;  y = normalised * pw + pb
   float mul[V][8], pw[V][8], add[kLayer ? V : 1][8], pb[kLayer ? V : 1][8];
   int col[V], n[V];
-  SavedPlace px[V], pbr[V], py[V];
+  int64_t step0[V];
   own_columns<V>(t, c, col, n);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    px[v] = saved_place(A.sx, col[v], c.d);
-    pbr[v] = saved_place(A.sb, col[v], c.d);
-    py[v] = saved_place(A.sy, col[v], c.d);
+    step0[v] = kSave ? first_step(c, col[v]) : 0;
     float w[8], g[8];
     param8(c.pre_w, col[v], c.d, 1.f, pw[v]);
     scale8(c, col[v], w);
@@ -279,8 +272,8 @@ __global__ void __launch_bounds__(kTypedThreads, V == 1 ? 2 : 1)
     const int r = live ? int(next) : 0;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      nx[v] = load_part<XT>(A.x, at(r, A.x.ld, col[v]), live ? n[v] : 0);
-      nb[v] = load_part<BT>(A.b, at(r, A.b.ld, col[v]), live && has_b ? n[v] : 0);
+      nx[v] = load_part<XT, kVec>(A.x, at(r, A.x.ld, col[v]), live ? n[v] : 0);
+      nb[v] = load_part<BT, kVec>(A.b, at(r, A.b.ld, col[v]), live && has_b ? n[v] : 0);
     }
   };
   fetch();
@@ -299,9 +292,9 @@ __global__ void __launch_bounds__(kTypedThreads, V == 1 ? 2 : 1)
     next += step;
     fetch();
     if (has_b) {
-      if (A.sb.codes) {
+      if (kSave && A.sb.codes) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) save_raw<BT>(A.sb, pbr[v], row, col[v], rb[v], b[v]);
+        for (int v = 0; v < V; ++v) save_raw<BT>(A.sb, c, step0[v], row, col[v], rb[v], b[v]);
       }
       if (c.post_norm) normalise_row<V, kLayer>(b, n, c, t, sums, turn);
 #pragma unroll
@@ -318,15 +311,15 @@ __global__ void __launch_bounds__(kTypedThreads, V == 1 ? 2 : 1)
             x[v][k] = fmaf(kLayer ? fmaf(b[v][k], mul[v][k], add[kLayer ? v : 0][k]) : b[v][k] * mul[v][k], g[k], x[v][k]);
         }
         rx[v] = pack<XT>(x[v]);
-        if (n[v]) store_part<XT>(A.x_out, at(row, A.x_out.ld, col[v]), n[v], rx[v]);
+        if (n[v]) store_part<XT, kVec>(A.x_out, at(row, A.x_out.ld, col[v]), n[v], rx[v]);
       }
     }
-    if (A.sx.codes) {
+    if (kSave && A.sx.codes) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         float f[8];
         unpack<XT>(rx[v], f);
-        save_raw<XT>(A.sx, px[v], row, col[v], rx[v], f);
+        save_raw<XT>(A.sx, c, step0[v], row, col[v], rx[v], f);
       }
     }
     if (!has_y) continue;
@@ -336,26 +329,26 @@ __global__ void __launch_bounds__(kTypedThreads, V == 1 ? 2 : 1)
 #pragma unroll
       for (int k = 0; k < 8; ++k) x[v][k] = kLayer ? fmaf(x[v][k], pw[v][k], pb[kLayer ? v : 0][k]) : x[v][k] * pw[v][k];
       const Raw8<BT> raw = pack<BT>(x[v]);
-      if (n[v]) store_part<BT>(A.y, at(row, A.y.ld, col[v]), n[v], raw);
-      if (A.sy.codes) {
+      if (n[v]) store_part<BT, kVec>(A.y, at(row, A.y.ld, col[v]), n[v], raw);
+      if (kSave && A.sy.codes) {
         unpack<BT>(raw, x[v]);
-        save_raw<BT>(A.sy, py[v], row, col[v], raw, x[v]);
+        save_raw<BT>(A.sy, c, step0[v], row, col[v], raw, x[v]);
       }
     }
   }
 }
 
 // One vector of x or b as it lies in memory: 8 elements, or 8 codes and a step.
-template <int DT, bool kSaved>
+template <int DT, bool kSaved, bool kVec>
 struct Held {
   Raw8<DT> raw;
   __device__ __forceinline__ void fetch(const RowView& t, const Saved8&, int64_t, int row, int col, int n) {
-    raw = load_part<DT>(t, at(row, t.ld, col), n);
+    raw = load_part<DT, kVec>(t, at(row, t.ld, col), n);
   }
   __device__ __forceinline__ void values(const Saved8&, float (&f)[8]) const { unpack<DT>(raw, f); }
 };
-template <int DT>
-struct Held<DT, true> {
+template <int DT, bool kVec>
+struct Held<DT, true, kVec> {
   uint2 codes;
   uint32_t step;
   __device__ __forceinline__ void fetch(const RowView&, const Saved8& s, int64_t step0, int row, int col, int n) {
@@ -371,7 +364,7 @@ struct Held<DT, true> {
   }
 };
 
-template <int XT, int BT, int V, bool kLayer, bool kSaved>
+template <int XT, int BT, int V, bool kLayer, bool kSaved, bool kVec>
 __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __grid_constant__ BwdArgs A, int team_threads) {
   constexpr int kSums = kLayer ? 4 : 2;  // P, R, then Q, U
   constexpr bool kAhead = V == 1;        // wider rows have no registers for the next one
@@ -391,7 +384,7 @@ __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __gri
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     param8(c.pre_w, col[v], c.d, 1.f, pw[v]);
-    step0[v] = kSaved && n[v] ? scale_index(A.sx.codes ? A.sx : A.sb, 0, col[v]) : 0;
+    step0[v] = kSaved ? first_step(c, col[v]) : 0;
   }
 
   for (int64_t item = blockIdx.x; item < A.items; item += gridDim.x) {
@@ -423,16 +416,16 @@ __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __gri
 
     Raw8<XT> ngx[V];
     Raw8<BT> ngy[V];
-    Held<XT, kSaved> nx[V];
-    Held<BT, kSaved> nb[V];
+    Held<XT, kSaved, kVec> nx[V];
+    Held<BT, kSaved, kVec> nb[V];
     auto fetch = [&](int r) {
       const bool in = r < last && r >= 0;  // r may pass 2^31 behind the last row
       const int row = in ? r : first;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const int live = in ? n[v] : 0;
-        ngx[v] = load_part<XT>(A.gx, at(row, A.gx.ld, col[v]), has_gx ? live : 0);
-        ngy[v] = load_part<BT>(A.gy, at(row, A.gy.ld, col[v]), has_y ? live : 0);
+        ngx[v] = load_part<XT, kVec>(A.gx, at(row, A.gx.ld, col[v]), has_gx ? live : 0);
+        ngy[v] = load_part<BT, kVec>(A.gy, at(row, A.gy.ld, col[v]), has_y ? live : 0);
         nx[v].fetch(A.x, A.sx, step0[v], row, col[v], has_y ? live : 0);
         nb[v].fetch(A.b, A.sb, step0[v], row, col[v], has_b ? live : 0);
       }
@@ -489,7 +482,7 @@ __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __gri
       }
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (n[v]) store_part<XT>(A.dx, at(row, A.dx.ld, col[v]), n[v], pack<XT>(e[v]));
+        if (n[v]) store_part<XT, kVec>(A.dx, at(row, A.dx.ld, col[v]), n[v], pack<XT>(e[v]));
       if (!has_b) continue;
 
       const float rb = c.post_norm ? factor(sbb, c) : 1.f;
@@ -553,7 +546,7 @@ __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __gri
       }
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (n[v]) store_part<BT>(A.db, at(row, A.db.ld, col[v]), n[v], pack<BT>(e[v]));
+        if (n[v]) store_part<BT, kVec>(A.db, at(row, A.db.ld, col[v]), n[v], pack<BT>(e[v]));
     }
 
     if (!A.partial) continue;
@@ -602,35 +595,39 @@ __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __gri
 }
 
 // An absent array, or one of this type with a stride that fits 32 bits.
-bool type_is(const RowView& t, int dt) { return !t.p || (t.dt == dt && t.ld <= 0x7FFFFFFF); }
-bool type_is(const RowOut& t, int dt) { return !t.p || (t.dt == dt && t.ld <= 0x7FFFFFFF); }
+template <typename View>
+bool type_is(const View& t, int dt) {
+  return !t.p || (t.dt == dt && t.ld <= 0x7FFFFFFF);
+}
+template <typename View>
+bool whole_vectors(const View& t) {
+  return !t.p || t.vec;
+}
 
-// Calls f with the pair of types and V as constants; false for another pair.
+// Calls f with the pair of types and whether rows are whole vectors as
+// constants; false for a combination that has no kernel.
 template <typename F>
-bool with_types(int xt, int bt, int vectors, F&& f) {
-  auto by_v = [&](auto x, auto b) {
-    if (vectors == 1) f(x, b, std::integral_constant<int, 1>{});
-    else f(x, b, std::integral_constant<int, 2>{});
-    return true;
-  };
+bool with_types(int xt, int bt, bool vec, F&& f) {
   using F32 = std::integral_constant<int, RF_F32>;
   using B16 = std::integral_constant<int, RF_BF16>;
   using F16 = std::integral_constant<int, RF_F16>;
-  if (xt == RF_BF16 && bt == RF_BF16) return by_v(B16{}, B16{});
-  if (xt == RF_F32 && bt == RF_BF16) return by_v(F32{}, B16{});
-  if (xt == RF_F32 && bt == RF_F32) return by_v(F32{}, F32{});
-  if (xt == RF_F16 && bt == RF_F16) return by_v(F16{}, F16{});
-  return false;
+  if (xt == RF_BF16 && bt == RF_BF16) vec ? f(B16{}, B16{}, std::true_type{}) : f(B16{}, B16{}, std::false_type{});
+  else if (xt == RF_F32 && bt == RF_F32) vec ? f(F32{}, F32{}, std::true_type{}) : f(F32{}, F32{}, std::false_type{});
+  else if (xt == RF_F32 && bt == RF_BF16 && vec) f(F32{}, B16{}, std::true_type{});
+  else if (xt == RF_F16 && bt == RF_F16 && vec) f(F16{}, F16{}, std::true_type{});
+  else return false;
+  return true;
+}
+
+TypedTeam team_for(int64_t d, int vectors) {
+  const int64_t nv = ceil_div(d, kPanel8) * (kPanel8 / 8);  // whole panels, for a saved row's last one
+  const int t = int(std::min<int64_t>(round_up(ceil_div(nv, vectors), 32), kTypedThreads));
+  return {t, vectors, std::min(kTypedThreads / t, kMaxTeams)};
 }
 
 }  // namespace
 
-TypedTeam typed_team(int64_t d) {
-  const int64_t nv = ceil_div(d, kPanel8) * (kPanel8 / 8);  // whole panels, for a saved row's last one
-  const int v = nv <= kTypedThreads ? 1 : 2;
-  const int t = int(std::min<int64_t>(round_up(ceil_div(nv, v), 32), kTypedThreads));
-  return {t, v, std::min(kTypedThreads / t, kMaxTeams)};
-}
+TypedTeam typed_team(int64_t d) { return team_for(d, d <= kMaxTyped / 2 ? 1 : 2); }
 
 bool try_typed_fwd(const rf_block_norm& p, const FwdArgs& A, cudaStream_t st) {
   const bool layer = p.kind == RF_LAYER_NORM;
@@ -638,14 +635,17 @@ bool try_typed_fwd(const rf_block_norm& p, const FwdArgs& A, cudaStream_t st) {
   if (p.features > kMaxTyped || !type_is(A.x, xt) || !type_is(A.b, bt) || !type_is(A.x_out, xt) || !type_is(A.y, bt) ||
       (!layer && (p.pre_bias.value || p.post_bias.value)))
     return false;
-  const TypedTeam t = typed_team(p.features);
-  const int64_t ctas = ceil_div(p.rows, t.teams);
-  const unsigned g = unsigned(std::min(ctas, int64_t(num_sms()) * (t.vectors == 1 ? 2 : 1)));
-  const unsigned b = unsigned(t.threads * t.teams);
-  return with_types(xt, bt, t.vectors, [&](auto x, auto y, auto v) {
-    constexpr int X = decltype(x)::value, B = decltype(y)::value, V = decltype(v)::value;
-    if (layer) k_norm_fwd_typed<X, B, V, true><<<g, b, 0, st>>>(A, t.threads);
-    else k_norm_fwd_typed<X, B, V, false><<<g, b, 0, st>>>(A, t.threads);
+  const bool vec = p.features % 8 == 0 && whole_vectors(A.x) && whole_vectors(A.b) && whole_vectors(A.x_out) &&
+                   whole_vectors(A.y);
+  const bool save = A.sx.codes || A.sb.codes || A.sy.codes;
+  const TypedTeam t = team_for(p.features, kFwdVectors);
+  const unsigned g = unsigned(std::min(ceil_div(p.rows, t.teams), int64_t(num_sms()))), b = unsigned(t.threads * t.teams);
+  return with_types(xt, bt, vec, [&](auto x, auto y, auto w) {
+    constexpr int X = decltype(x)::value, B = decltype(y)::value;
+    constexpr bool W = decltype(w)::value;
+    auto go = [&](auto kernel) { kernel<<<g, b, 0, st>>>(A, t.threads); };
+    if (layer) save ? go(k_norm_fwd_typed<X, B, true, true, W>) : go(k_norm_fwd_typed<X, B, true, false, W>);
+    else save ? go(k_norm_fwd_typed<X, B, false, true, W>) : go(k_norm_fwd_typed<X, B, false, false, W>);
   });
 }
 
@@ -654,17 +654,23 @@ bool try_typed_bwd(const rf_block_norm& p, const BwdArgs& A, bool bias, cudaStre
   const bool saved = A.sx.codes || A.sb.codes;
   const int xt = A.dx.dt, bt = A.db.p ? A.db.dt : A.gy.p ? A.gy.dt : xt;
   if (p.features > kMaxTyped || (!layer && bias) || !type_is(A.gx, xt) || !type_is(A.gy, bt) || !type_is(A.x, xt) ||
-      !type_is(A.b, bt) || (saved && (A.x.p || A.b.p)))
+      !type_is(A.b, bt) || (saved && (A.x.p || A.b.p)) || !type_is(A.dx, xt) || !type_is(A.db, bt))
     return false;
+  const bool vec = p.features % 8 == 0 && whole_vectors(A.gx) && whole_vectors(A.gy) && whole_vectors(A.x) &&
+                   whole_vectors(A.b) && whole_vectors(A.dx) && whole_vectors(A.db);
   const TypedTeam t = typed_team(p.features);
   const unsigned g = unsigned(std::min<int64_t>(A.items, 148 * 32)), b = unsigned(t.threads * t.teams);
   const size_t smem = t.teams > 1 ? size_t(layer ? 4 : 2) * t.threads * 8 * t.vectors * 4 : 0;  // at most 32 KB
-  return with_types(xt, bt, t.vectors, [&](auto x, auto y, auto v) {
-    constexpr int X = decltype(x)::value, B = decltype(y)::value, V = decltype(v)::value;
-    if (layer) saved ? k_norm_bwd_typed<X, B, V, true, true><<<g, b, smem, st>>>(A, t.threads)
-                     : k_norm_bwd_typed<X, B, V, true, false><<<g, b, smem, st>>>(A, t.threads);
-    else saved ? k_norm_bwd_typed<X, B, V, false, true><<<g, b, smem, st>>>(A, t.threads)
-               : k_norm_bwd_typed<X, B, V, false, false><<<g, b, smem, st>>>(A, t.threads);
+  return with_types(xt, bt, vec, [&](auto x, auto y, auto w) {
+    constexpr int X = decltype(x)::value, B = decltype(y)::value;
+    constexpr bool W = decltype(w)::value;
+    auto go = [&](auto kernel) { kernel<<<g, b, smem, st>>>(A, t.threads); };
+    auto by_v = [&](auto v) {
+      constexpr int V = decltype(v)::value;
+      if (layer) saved ? go(k_norm_bwd_typed<X, B, V, true, true, W>) : go(k_norm_bwd_typed<X, B, V, true, false, W>);
+      else saved ? go(k_norm_bwd_typed<X, B, V, false, true, W>) : go(k_norm_bwd_typed<X, B, V, false, false, W>);
+    };
+    t.vectors == 1 ? by_v(std::integral_constant<int, 1>{}) : by_v(std::integral_constant<int, 2>{});
   });
 }
 
