@@ -38,7 +38,7 @@ class SavedActivation:
     ``format``.  value = code * 2^(scale - 127), a scale of 255 meaning NaN;
     the scale of feature f is ``scales[f // 128, row, f % 128 // 32]``."""
 
-    __slots__ = ("codes", "scales", "shape", "dtype", "format", "rows", "features")
+    __slots__ = ("_codes", "_scales", "_buffer", "shape", "dtype", "format", "rows", "features")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, dtype: torch.dtype, format: str):
         _format_code(format)
@@ -53,12 +53,47 @@ class SavedActivation:
                                  f"got {tuple(t.shape)}")
         if codes.device != scales.device:
             raise ValueError("codes and scales must be on one device")
-        self.codes, self.scales, self.shape, self.dtype, self.format = codes, scales, shape, dtype, format
-        self.rows, self.features = rows, features
+        self._codes, self._scales, self._buffer = codes, scales, None
+        self.shape, self.dtype, self.format, self.rows, self.features = shape, dtype, format, rows, features
+
+    @classmethod
+    def _empty(cls, shape, dtype, format, device) -> "SavedActivation":
+        """One allocation for codes and scales; their tensors are made when
+        someone asks for them."""
+        self = object.__new__(cls)
+        self.rows, self.features = rows, features = _rows_features(shape, "a saved activation")
+        self.shape, self.dtype, self.format = shape, dtype, format
+        self._codes = self._scales = None
+        self._buffer = torch.empty(_up(rows * _up(features, 16), 256) + -(-features // 128) * _up(rows, 64) * 4,
+                                   dtype=torch.uint8, device=device)
+        return self
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            ld = _up(self.features, 16)
+            self._codes = self._buffer[:self.rows * ld].view(self.rows, ld)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._buffer[_up(self.rows * _up(self.features, 16), 256):].view(
+                -(-self.features // 128), _up(self.rows, 64), 4)
+        return self._scales
+
+    def _native(self) -> _lib.RfSavedActivation:
+        ld, code = _up(self.features, 16), _lib.FORMAT8_CODES[self.format]
+        if self._buffer is not None:
+            codes = self._buffer.data_ptr()
+            scales = codes + _up(self.rows * ld, 256)
+        else:
+            codes, scales = self._codes.data_ptr(), self._scales.data_ptr()
+        return _lib.RfSavedActivation(codes, scales, self.rows, self.features, ld, _up(self.rows, 64), code)
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return (self._codes if self._buffer is None else self._buffer).device
 
     @property
     def nbytes(self) -> int:
@@ -118,23 +153,19 @@ def _out_rows(t: torch.Tensor, what: str) -> int:
     return ld
 
 
-@contextlib.contextmanager
-def _other_device(device: torch.device):
-    with torch.cuda.device(device):
-        yield
-
-
 _here = contextlib.nullcontext()
 
 
 def on_device(device: torch.device):
     """A launch must come from the arrays' device; switching costs more than
     the check that it is current already."""
-    return _here if device.index == torch.cuda.current_device() else _other_device(device)
+    return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def stream_of(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """Handle of the current stream, without a Stream object: that takes
+    microseconds, as much as a small call's launch."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def require_same_device(device: torch.device, **tensors) -> None:
@@ -145,28 +176,19 @@ def require_same_device(device: torch.device, **tensors) -> None:
 
 def native(saved: SavedActivation | None):
     """The ctypes form, or None."""
-    if saved is None:
-        return None
-    return ctypes.byref(native_struct(saved))
-
-
-def native_struct(saved: SavedActivation) -> _lib.RfSavedActivation:
-    return _lib.RfSavedActivation(saved.codes.data_ptr(), saved.scales.data_ptr(), saved.rows, saved.features,
-                                  saved.codes.shape[1], saved.scales.shape[1], _lib.FORMAT8_CODES[saved.format])
+    return None if saved is None else saved._native()
 
 
 def empty_saved(shape, dtype: torch.dtype, format: str, device: torch.device) -> SavedActivation:
-    rows, features = _rows_features(tuple(shape), "a saved activation")
     _format_code(format)
-    return SavedActivation(torch.empty((rows, _up(features, 16)), dtype=torch.uint8, device=device),
-                           torch.empty((-(-features // 128), _up(rows, 64), 4), dtype=torch.uint8, device=device),
-                           shape, dtype, format)
+    return SavedActivation._empty(tuple(shape), dtype, format, device)
 
 
 def _require_saved(saved, what: str) -> None:
     if not isinstance(saved, SavedActivation):
         raise ValueError(f"{what} must be a SavedActivation, got {type(saved).__name__}")
-    require_cuda(saved.codes, what)
+    if saved.device.type != "cuda":
+        require_cuda(saved.codes, what)
 
 
 def _check_seed(seed) -> int:

@@ -26,7 +26,7 @@ import torch
 
 from . import _lib
 from .activations import (SavedActivation, _format_code, _require_saved, _rows_features, empty_saved, native,
-                          native_struct, on_device, require_same_device, row_strided, stream_of)
+                          on_device, require_same_device, row_strided, stream_of)
 from .base import require_cuda, rf_dtype
 
 _KINDS = {"rms": _lib.RF_RMS_NORM, "layer": _lib.RF_LAYER_NORM}
@@ -122,7 +122,7 @@ def _rows(t, what: str, shape):
         _require_saved(t, what)
         if t.shape != shape:
             raise ValueError(f"{what} must have shape {shape}, got {t.shape}")
-        s = native_struct(t)
+        s = t._native()
         return _lib.RfRows(None, 0, 0, ctypes.pointer(s)), (t, s)
     require_cuda(t, what)
     if tuple(t.shape) != shape:

@@ -17,6 +17,7 @@
 #include "rf_act8.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "rf_kernels.cuh"
@@ -50,16 +51,23 @@ constexpr int kThreads = 256;
 struct Walk {
   dim3 block, grid;
 };
-template <typename Kernel>
-Walk walk(Kernel kernel, int64_t rows, int64_t features, int rows_per_thread, int elements = 8) {
+template <auto kernel>
+Walk walk(int64_t rows, int64_t features, int rows_per_thread, int elements = 8) {
   const int64_t nv = ceil_div(features, kPanel8) * (kPanel8 / elements);
   const int tx = int(nv >= kThreads ? kThreads : nv == 16 ? 16 : round_up(nv, 32));
   const int ty = kThreads / tx;
   const int64_t gy = ceil_div(nv, tx), tiles = ceil_div(rows, int64_t(ty) * rows_per_thread);
-  int per_sm = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, tx * ty, 0) != cudaSuccess || per_sm < 1) {
-    cudaGetLastError();
-    per_sm = 2;
+  // Asked once per kernel (and block size: whole warps up to 256 threads): the
+  // answer is the same on every GPU of the kind, and asking takes microseconds.
+  static std::atomic<int> asked[kThreads / 32 + 1];
+  std::atomic<int>& known = asked[tx * ty / 32];
+  int per_sm = known.load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, tx * ty, 0) != cudaSuccess || per_sm < 1) {
+      cudaGetLastError();
+      per_sm = 2;
+    }
+    known.store(per_sm, std::memory_order_relaxed);
   }
   // Three CTAs per SM: 16384 x 14336 saved in 117 us; with two or four 131.
   const int64_t held = std::max<int64_t>(1, int64_t(num_sms()) * std::min(per_sm, 3) / gy);
@@ -633,11 +641,12 @@ extern "C" rf_status rf_save_activation(const void* x, int64_t ldx, int32_t dtyp
   if (typed(out->features, x, ldx, dtype)) {
     with_types(dtype, out->format, [&](auto dt, auto fmt) {
       constexpr int DT = decltype(dt)::value, F = decltype(fmt)::value, R = DT == RF_F32 ? 2 : 4;
-      auto go = [&](auto kernel) {
-        const Walk w = walk(kernel, out->rows, out->features, R);
+      auto go = [&](auto sr) {
+        constexpr auto kernel = k_save_typed<DT, F, decltype(sr)::value>;
+        const Walk w = walk<kernel>(out->rows, out->features, R);
         kernel<<<w.grid, w.block, 0, st>>>(x, ldx, saved8(*out), out->rows, out->features, seed);
       };
-      stochastic ? go(k_save_typed<DT, F, true>) : go(k_save_typed<DT, F, false>);
+      stochastic ? go(std::true_type{}) : go(std::false_type{});
     });
     return check_launch("k_save");
   }
@@ -658,8 +667,8 @@ extern "C" rf_status rf_load_activation(const rf_saved_activation* saved, void* 
   if (typed(saved->features, out, ldo, dtype)) {
     with_types(dtype, saved->format, [&](auto dt, auto fmt) {
       constexpr int DT = decltype(dt)::value;
-      auto kernel = k_load_typed<DT, decltype(fmt)::value>;
-      const Walk w = walk(kernel, saved->rows, saved->features, 4, DT == RF_F32 ? 4 : 8);
+      constexpr auto kernel = k_load_typed<DT, decltype(fmt)::value>;
+      const Walk w = walk<kernel>(saved->rows, saved->features, 4, DT == RF_F32 ? 4 : 8);
       kernel<<<w.grid, w.block, 0, st>>>(saved8(*saved), out, ldo, saved->rows, saved->features);
     });
     return check_launch("k_load");
@@ -695,11 +704,12 @@ extern "C" rf_status rf_swiglu_forward(const void* gate, int64_t ld_gate, const 
       (!saved_gate || saved_gate->format == saved_up->format)) {
     with_types(dtype, saved_gate ? saved_gate->format : int32_t(RF_INT8), [&](auto dt, auto fmt) {
       constexpr int DT = decltype(dt)::value, F = decltype(fmt)::value, R = DT == RF_F32 ? 1 : 2;
-      auto go = [&](auto kernel) {
-        const Walk w = walk(kernel, rows, features, R);
+      auto go = [&](auto save) {
+        constexpr auto kernel = k_swiglu_fwd_typed<DT, F, decltype(save)::value>;
+        const Walk w = walk<kernel>(rows, features, R);
         kernel<<<w.grid, w.block, 0, st>>>(gate, ld_gate, up, ld_up, h, ld_h, sg, su, rows, features);
       };
-      saved_gate ? go(k_swiglu_fwd_typed<DT, F, true>) : go(k_swiglu_fwd_typed<DT, F, false>);
+      saved_gate ? go(std::true_type{}) : go(std::false_type{});
     });
     return check_launch("k_swiglu_fwd");
   }
@@ -736,12 +746,13 @@ extern "C" rf_status rf_swiglu_backward(const void* grad_h, int64_t ld_grad, con
       typed(features, grad_up, ld_up, dtype)) {
     with_types(dtype, saved_h ? saved_h->format : int32_t(RF_INT8), [&](auto dt, auto fmt) {
       constexpr int DT = decltype(dt)::value, F = decltype(fmt)::value, R = 1;
-      auto go = [&](auto kernel) {
-        const Walk w = walk(kernel, rows, features, R);
+      auto go = [&](auto save) {
+        constexpr auto kernel = k_swiglu_bwd_typed<DT, F, decltype(save)::value>;
+        const Walk w = walk<kernel>(rows, features, R);
         kernel<<<w.grid, w.block, 0, st>>>(grad_h, ld_grad, saved8(*saved_gate), saved8(*saved_up), grad_gate, ld_gate,
                                            grad_up, ld_up, sh, rows, features);
       };
-      saved_h ? go(k_swiglu_bwd_typed<DT, F, true>) : go(k_swiglu_bwd_typed<DT, F, false>);
+      saved_h ? go(std::true_type{}) : go(std::false_type{});
     });
     return check_launch("k_swiglu_bwd");
   }
