@@ -273,6 +273,8 @@ __global__ void __launch_bounds__(kThreads) k_save_typed(const void* x, int64_t 
 template <int DT, int kFormat>
 __global__ void __launch_bounds__(kThreads) k_load_typed(Saved8 in, void* out, int64_t ldo, int64_t rows,
                                                          int64_t features) {
+  // The weight gradient's products may set up while this drains.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr int R = 4, E = DT == RF_F32 ? 4 : 8;
   const int64_t col = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * E;
   if (col >= features) return;  // widths here are multiples of 8

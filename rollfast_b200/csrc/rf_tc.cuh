@@ -200,6 +200,10 @@ __device__ __forceinline__ bool mbar_wait_short(uint32_t bar, uint32_t parity, v
     }
   }
 }
+// Programmatic dependent launch: a kernel launched with launch_dependent may
+// start while the previous one drains, and touches what that one writes only
+// behind prior_kernel_done (at once for a plain launch).
+__device__ __forceinline__ void prior_kernel_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Bounded wait without a result, before a role ends.
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
   const uint64_t t0 = globaltimer();

@@ -35,6 +35,7 @@
 // tiles a second kernel adds in a fixed order.
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "rf_act8.cuh"
 #include "rf_kernels.cuh"
@@ -59,6 +60,7 @@ constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kFirstEpilogue = 4, kEpilogueWarps = 8;  // a multiple of 4: a warp reads TMEM lanes 32 (warp % 4) ..
 constexpr int kThreads = (kFirstEpilogue + kEpilogueWarps) * 32;
 constexpr int kColumns = kTile / (kEpilogueWarps / 4);  // accumulator columns per epilogue warp
+static_assert(kColumns == 128, "the epilogue names its eight blocks of 16");
 constexpr int kStagingFloats = 32 * 16;                 // a warp's 32 x 16 block on its way out
 constexpr int kStagingOff = kStages * kStageBytes;
 constexpr int kBarOff = kStagingOff + kEpilogueWarps * kStagingFloats * 4;
@@ -154,49 +156,59 @@ __device__ __forceinline__ float4 add4(float4 a, float4 b) {
   return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
 }
 
-// A warp's 32 x 16 block, lane = row in v[], through its staging buffer, so
-// that a store instruction covers 8 rows of 64 bytes.  16-byte chunk c of row
-// r lies at c ^ (r / 2 % 4): both the row writes and the reads of 8 rows by 4
-// chunks touch every bank once.  The initial values of a block are loaded
-// together, ahead of their use: one at a time, their latency outlasted the
-// next tile's products.
-__device__ __forceinline__ void store_block(const Params& P, float* part, int64_t row0, int64_t col0, int lane,
-                                            const float* v, float* stg) {
-  const int r0 = lane >> 2;
-  const int64_t col = col0 + 4 * (lane & 3);
-  const int64_t live = P.n - col;
-  const bool vec = P.vec && live >= 4;
-  const int64_t ld = part ? kTile : P.ld_out;
-  const int64_t i = part ? (row0 + r0) % kTile * kTile + col % kTile : (row0 + r0) * P.ld_out + col;
-  const int rows = int(min(P.m - row0 - r0, int64_t(32)));  // this lane's row r0 + 8 it is inside while 8 it < rows
-  float4 a[4];
-#pragma unroll
-  for (int it = 0; it < 4; ++it) {
-    a[it] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (!part && P.initial && vec && 8 * it < rows) a[it] = initial4(P, i + 8 * it * ld);
-  }
-  __syncwarp();
+// A warp's 32 x 16 block of sums, lane = row, goes through its staging buffer,
+// so that a store instruction covers 8 rows of 64 bytes.  16-byte chunk c of
+// row r lies at c ^ (r / 2 % 4): both the row writes and the reads of 8 rows
+// by 4 chunks touch every bank once.
+__device__ __forceinline__ void stage_block(int lane, const float* v, float* stg) {
 #pragma unroll
   for (int c = 0; c < 4; ++c)
     *reinterpret_cast<float4*>(stg + lane * 16 + ((c ^ ((lane >> 1) & 3)) << 2)) =
         make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-  __syncwarp();
-  if (live <= 0) return;
-  // Row r0 + 8 it: r / 2 % 4 is that of r0.
-  const float* src = stg + r0 * 16 + (((lane & 3) ^ ((r0 >> 1) & 3)) << 2);
+}
+// The initial values of a block, loaded together and ahead of the staging: one
+// at a time, their latency outlasted the next tile's products.
+struct BlockAt {
+  int64_t i, ld, live;
+  int rows;  // this lane's row r + 8 it is inside while 8 it < rows
+  bool vec;
+  float4 initial[4];
+};
+__device__ __forceinline__ BlockAt block_at(const Params& P, const float* part, int64_t row0, int64_t col0, int lane) {
+  BlockAt b;
+  const int r = lane >> 2;
+  const int64_t col = col0 + 4 * (lane & 3);
+  b.live = P.n - col;
+  b.vec = P.vec && b.live >= 4;
+  b.ld = part ? kTile : P.ld_out;
+  b.i = part ? (row0 + r) % kTile * kTile + col % kTile : (row0 + r) * P.ld_out + col;
+  b.rows = b.live > 0 ? int(min(P.m - row0 - r, int64_t(32))) : 0;
 #pragma unroll
   for (int it = 0; it < 4; ++it) {
-    if (8 * it >= rows) break;
+    b.initial[it] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!part && P.initial && b.vec && 8 * it < b.rows) b.initial[it] = initial4(P, b.i + 8 * it * b.ld);
+  }
+  return b;
+}
+__device__ __forceinline__ void store_block(const Params& P, float* part, const BlockAt& b, int lane, const float* stg) {
+  const int r = lane >> 2;  // row r + 8 it: its / 2 % 4 is that of r
+  const float* src = stg + r * 16 + (((lane & 3) ^ ((r >> 1) & 3)) << 2);
+#pragma unroll
+  for (int it = 0; it < 4; ++it) {
+    if (8 * it >= b.rows) break;
     const float4 x = *reinterpret_cast<const float4*>(src + 128 * it);
-    if (part) *reinterpret_cast<float4*>(part + i + 8 * it * ld) = x;
-    else if (vec) put4(P, i + 8 * it * ld, add4(x, a[it]));
-    else add_put_each(P, i + 8 * it * ld, live, x);
+    const int64_t i = b.i + 8 * it * b.ld;
+    if (part) *reinterpret_cast<float4*>(part + i) = x;
+    else if (b.vec) put4(P, i, add4(x, b.initial[it]));
+    else add_put_each(P, i, b.live, x);
   }
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     k_weight_grad(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_g,
                   const __grid_constant__ Params P) {
+  // The join's CTAs may take the SMs that this grid leaves.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBarOff);
@@ -241,6 +253,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // ---------------- loads (both CTAs, each its own halves) ----------------
       // A warp for each operand: a wait and four copies take one thread about
       // as long as the products of a step.
+      prior_kernel_done();  // X and the terms of G are complete
       const bool x = warp == 0;
       const CUtensorMap* map = x ? &tm_x : &tm_g;
       int stage = 0;
@@ -386,11 +399,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int64_t row0 = int64_t(I) * kTile + int64_t(rank) * kHalf + quarter * 32;
       const int64_t col0 = int64_t(J) * kTile + first_col;
       float* dst = part < 0 ? nullptr : P.partial + part * (kTile * kTile);
-      if (row0 < P.m) {
-#pragma unroll
-        for (int c = 0; c < kColumns; c += 16) {
-          if (col0 + c < P.n) store_block(P, dst, row0, col0 + c, lane, sum + c, stg);
+      // Whole float32 blocks to a partial tile or an output without initial
+      // values: four reads, four stores.
+      float* plain = dst ? dst + (row0 % kTile + (lane >> 2)) * kTile + first_col + 4 * (lane & 3)
+                         : static_cast<float*>(P.out) + (row0 + (lane >> 2)) * P.ld_out + col0 + 4 * (lane & 3);
+      const int64_t plain_ld = 8 * (dst ? kTile : P.ld_out);
+      const bool fast = (dst || (P.vec && P.out_dt == RF_F32 && !P.initial)) && row0 + 32 <= P.m;
+      // One copy of the store's code for all blocks (unrolled, it did not fit
+      // the instruction cache: 17 us a tile); only the registers that a block
+      // comes from are spelled out.
+#pragma unroll 1
+      for (int c = 0; c < kColumns / 16; ++c) {
+        if (row0 >= P.m || col0 + 16 * c >= P.n) break;
+        const bool simple = fast && col0 + 16 * c + 16 <= P.n;
+        BlockAt at;
+        if (!simple) at = block_at(P, dst, row0, col0 + 16 * c, lane);
+        switch (c) {
+          case 0: stage_block(lane, sum, stg); break;
+          case 1: stage_block(lane, sum + 16, stg); break;
+          case 2: stage_block(lane, sum + 32, stg); break;
+          case 3: stage_block(lane, sum + 48, stg); break;
+          case 4: stage_block(lane, sum + 64, stg); break;
+          case 5: stage_block(lane, sum + 80, stg); break;
+          case 6: stage_block(lane, sum + 96, stg); break;
+          default: stage_block(lane, sum + 112, stg); break;
         }
+        __syncwarp();
+        if (simple) {
+          const float* src = stg + (lane >> 2) * 16 + (((lane & 3) ^ ((lane >> 3) & 3)) << 2);
+          float4 x[4];
+#pragma unroll
+          for (int it = 0; it < 4; ++it) x[it] = *reinterpret_cast<const float4*>(src + 128 * it);
+#pragma unroll
+          for (int it = 0; it < 4; ++it) *reinterpret_cast<float4*>(plain + it * plain_ld + 16 * c) = x[it];
+        } else {
+          store_block(P, dst, at, lane, stg);
+        }
+        __syncwarp();
       }
     }
   }
@@ -411,6 +456,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // cut from an infinity or a NaN stays alone (the others are 0).
 __global__ void __launch_bounds__(256) k_grad_terms(RowView g, uint16_t* out, int64_t rows, int64_t n, int64_t ld,
                                                     int terms) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t col = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 8;
   if (col >= ld) return;
   for (int64_t row = int64_t(blockIdx.x) * blockDim.y + threadIdx.y; row < rows; row += int64_t(gridDim.x) * blockDim.y) {
@@ -441,6 +487,7 @@ __global__ void __launch_bounds__(256) k_weight_grad_join(const __grid_constant_
   tile_at(P.whole + tail, P.tiles_i, P.tiles_j, I, J);
   const int64_t row = int64_t(I) * kTile + r, col = int64_t(J) * kTile + c;
   if (row >= P.m || col >= P.n) return;
+  prior_kernel_done();
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   const float* p = P.partial + tail * P.splits * (kTile * kTile) + r * kTile + c;
 #pragma unroll 4
@@ -494,6 +541,25 @@ Tail choose_tail(int64_t tiles, int64_t steps, int64_t pairs) {
   }
   if (t.splits == 1) t.whole = tiles;
   return t;
+}
+
+// A kernel that starts while the one before it drains (rf_tc.cuh).
+template <typename... Args>
+rf_status launch_dependent(void (*kernel)(Args...), unsigned grid, int threads, int smem, cudaStream_t st,
+                           const std::decay_t<Args>&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return fail(RF_ECUDA, std::string("rf_weight_gradient launch: ") + cudaGetErrorString(e));
+  return check_launch("rf_weight_gradient");
 }
 
 struct Plan {
@@ -659,10 +725,8 @@ extern "C" rf_status rf_weight_gradient(const rf_saved_activation* saved, const 
     RF_TRY(make_map(&mg, g, n_out, rows, p.terms, ldg));
     RF_TRY(allow_smem());
     const int64_t pairs = std::min(P.units, max_pairs());
-    k_weight_grad<<<unsigned(2 * pairs), kThreads, kSmemBytes, st>>>(mx, mg, P);
-    RF_TRY(check_launch("k_weight_grad"));
+    RF_TRY(launch_dependent(k_weight_grad, unsigned(2 * pairs), kThreads, kSmemBytes, st, mx, mg, P));
   }
   if (P.whole == tiles) return RF_OK;
-  k_weight_grad_join<<<unsigned((tiles - P.whole) * (kTile / 4)), 256, 0, st>>>(P);
-  return check_launch("k_weight_grad_join");
+  return launch_dependent(k_weight_grad_join, unsigned((tiles - P.whole) * (kTile / 4)), 256, 0, st, P);
 }
