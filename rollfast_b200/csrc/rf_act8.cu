@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kThreads) k_load_typed(Saved8 in, void* out, i
       decode4(w[r].x, kFormat, f);
       if (E == 8) decode4(w[r].y, kFormat, f + 4);
 #pragma unroll
-      for (int k = 0; k < E; ++k) f[k] *= st[r];
+      for (int k = 0; k < E / 2; ++k) put_pair(f, k, __fmul2_rn(pair(f, k), both(st[r])));
       if (E == 8) {
         saturate8(DT, f);
         to.store(r, f);
@@ -433,7 +433,9 @@ __global__ void __launch_bounds__(kThreads) k_swiglu_fwd_typed(const void* gate,
         }
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) g[k] = g[k] * sigmoid(g[k]) * u[k];
+      for (int k = 0; k < 4; ++k)
+        put_pair(g, k, __fmul2_rn(__fmul2_rn(pair(g, k), make_float2(sigmoid(g[2 * k]), sigmoid(g[2 * k + 1]))),
+                                  pair(u, k)));
       if (data && r < n) ch.store(r, g);
     }
     n = after;
@@ -447,13 +449,14 @@ __global__ void __launch_bounds__(kThreads) k_swiglu_fwd_typed(const void* gate,
 // the gradients.
 __device__ __forceinline__ void swiglu_back8(const float (&d)[8], float (&g)[8], float (&u)[8], float (&h)[8]) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const float s = sigmoid(g[k]);
-    const float a = g[k] * s;
-    h[k] = a * u[k];
-    const float slope = fmaf(a, 1.f - s, s);
-    g[k] = d[k] * u[k] * slope;
-    u[k] = d[k] * a;
+  for (int k = 0; k < 4; ++k) {
+    const float2 s = make_float2(sigmoid(g[2 * k]), sigmoid(g[2 * k + 1]));
+    const float2 x = pair(u, k), y = pair(d, k);
+    const float2 a = __fmul2_rn(pair(g, k), s);
+    put_pair(h, k, __fmul2_rn(a, x));
+    const float2 slope = __ffma2_rn(a, __ffma2_rn(s, both(-1.f), both(1.f)), s);
+    put_pair(g, k, __fmul2_rn(__fmul2_rn(y, x), slope));
+    put_pair(u, k, __fmul2_rn(y, a));
   }
 }
 
@@ -513,11 +516,8 @@ __global__ void __launch_bounds__(kThreads) k_swiglu_bwd_typed(const void* dh, i
       decode4(rg[r].y, gate.format, g + 4);
       decode4(ru[r].x, up.format, u);
       decode4(ru[r].y, up.format, u + 4);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        g[k] *= fg[r];
-        u[k] *= fu[r];
-      }
+      mul8(g, both(fg[r]));
+      mul8(u, both(fu[r]));
       swiglu_back8(d, g, u, h);
       if (kSave) {
         const uint32_t b = step_byte(block_max_bits(h), kFormat);

@@ -195,6 +195,24 @@ __device__ __forceinline__ void store_vec(void* p, int64_t i, const float (&f)[8
   }
 }
 
+// -- pairs ------------------------------------------------------------------
+// sm_100 multiplies and adds two float32 in one instruction; these kernels are
+// short of issue slots, not of arithmetic.  Same roundings as one by one.
+__device__ __forceinline__ float2 pair(const float* f, int k) { return make_float2(f[2 * k], f[2 * k + 1]); }
+__device__ __forceinline__ void put_pair(float* f, int k, float2 v) {
+  f[2 * k] = v.x;
+  f[2 * k + 1] = v.y;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ void mul8(float (&f)[8], float2 s) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) put_pair(f, k, __fmul2_rn(pair(f, k), s));
+}
+__device__ __forceinline__ void mul8(float (&f)[8], const float (&g)[8]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) put_pair(f, k, __fmul2_rn(pair(f, k), pair(g, k)));
+}
+
 // -- codes ------------------------------------------------------------------
 __device__ __forceinline__ float step_value(uint32_t s) {
   return __uint_as_float(s == kNanStep ? 0x7FC00000u : s << 23);
@@ -205,10 +223,11 @@ __device__ __forceinline__ void decode4(uint32_t w, int format, float* f) {
   if (format == RF_INT8) {
     // q + 128 in the low byte of 2^23's significand, then an exact subtraction.
     const uint32_t o = w ^ 0x80808080u;
-    f[0] = __uint_as_float(__byte_perm(o, 0x4B000000u, 0x7650)) - 8388736.f;
-    f[1] = __uint_as_float(__byte_perm(o, 0x4B000000u, 0x7651)) - 8388736.f;
-    f[2] = __uint_as_float(__byte_perm(o, 0x4B000000u, 0x7652)) - 8388736.f;
-    f[3] = __uint_as_float(__byte_perm(o, 0x4B000000u, 0x7653)) - 8388736.f;
+    const float2 off = both(-8388736.f);
+    put_pair(f, 0, __fadd2_rn(make_float2(__uint_as_float(__byte_perm(o, 0x4B000000u, 0x7650)),
+                                          __uint_as_float(__byte_perm(o, 0x4B000000u, 0x7651))), off));
+    put_pair(f, 1, __fadd2_rn(make_float2(__uint_as_float(__byte_perm(o, 0x4B000000u, 0x7652)),
+                                          __uint_as_float(__byte_perm(o, 0x4B000000u, 0x7653))), off));
   } else {
     const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(w & 0xFFFFu), __NV_E4M3);
     const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(w >> 16), __NV_E4M3);
@@ -232,8 +251,7 @@ __device__ __forceinline__ void load8(const Saved8& s, int64_t row, int64_t col,
   const float st = step_value(__ldg(s.scales + scale_index(s, row, col)));
   decode4(w.x, s.format, f);
   decode4(w.y, s.format, f + 4);
-#pragma unroll
-  for (int k = 0; k < 8; ++k) f[k] *= st;
+  mul8(f, both(st));
 }
 
 // The step byte for a block whose largest magnitude has the float bits `a`
@@ -287,8 +305,11 @@ __device__ __forceinline__ uint2 encode8(const float (&f)[8], uint32_t s, int fo
       for (int k = 0; k < 8; ++k) b[k] = __float_as_uint(fminf(fmaxf(f[k] * inv, -127.f), 127.f) + 12582912.f);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)  // adding 1.5 * 2^23 rounds to an integer, whose low byte is the code
-        b[k] = __float_as_uint(fmaf(f[k], inv, 12582912.f));
+      for (int k = 0; k < 4; ++k) {  // adding 1.5 * 2^23 rounds to an integer, whose low byte is the code
+        const float2 r = __ffma2_rn(pair(f, k), both(inv), both(12582912.f));
+        b[2 * k] = __float_as_uint(r.x);
+        b[2 * k + 1] = __float_as_uint(r.y);
+      }
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -297,10 +318,10 @@ __device__ __forceinline__ uint2 encode8(const float (&f)[8], uint32_t s, int fo
   } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * h] * inv, f[4 * h + 1] * inv), __NV_SATFINITE,
-                                                   __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * h + 2] * inv, f[4 * h + 3] * inv),
-                                                   __NV_SATFINITE, __NV_E4M3);
+      const uint32_t lo =
+          __nv_cvt_float2_to_fp8x2(__fmul2_rn(pair(f, 2 * h), both(inv)), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi =
+          __nv_cvt_float2_to_fp8x2(__fmul2_rn(pair(f, 2 * h + 1), both(inv)), __NV_SATFINITE, __NV_E4M3);
       w[h] = lo | (hi << 16);
     }
   }

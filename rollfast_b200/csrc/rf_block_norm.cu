@@ -354,10 +354,10 @@ struct ColArgs {
   float* gate_cols;          // [groups][ldp]: summands of a scalar gate's gradient
   float* scale_cols;         // [ldp]: summands of a scalar scale's gradient
 };
-constexpr int kColLanes = 16;
+constexpr int kColLanes = 32;
 
 __global__ void __launch_bounds__(32 * kColLanes) k_norm_cols(const __grid_constant__ ColArgs A) {
-  __shared__ float sm[5][kColLanes][33];
+  __shared__ float sm[4][kColLanes][33];
   const Common& c = A.c;
   const int tx = int(threadIdx.x) & 31, ty = int(threadIdx.x) >> 5;
   const int64_t col = int64_t(blockIdx.x) * 32 + tx;
@@ -402,22 +402,23 @@ __global__ void __launch_bounds__(32 * kColLanes) k_norm_cols(const __grid_const
       add_items(g * A.chunks, (g + 1) * A.chunks, 1, p, q);
       close_group(g, p, q);
     }
-  } else {
-    for (int64_t g = 0; g < A.groups; ++g) {
-      float p = 0.f, q = 0.f;
-      add_items(g * A.chunks + ty, (g + 1) * A.chunks, kColLanes, p, q);
-      sm[0][ty][tx] = p;
-      sm[1][ty][tx] = q;
-      __syncthreads();
-      if (ty == 0) {
-        for (int k = 1; k < kColLanes; ++k) {
-          p += sm[0][k][tx];
-          q += sm[1][k][tx];
-        }
-        close_group(g, p, q);
+  } else if (A.groups > 0) {
+    // Few groups: each gets a share of the lanes, whose parts its first lane adds.
+    const int share = kColLanes / int(A.groups);
+    const int g = ty / share, j = ty - g * share;
+    float p = 0.f, q = 0.f;
+    if (g < A.groups) add_items(g * A.chunks + j, (int64_t(g) + 1) * A.chunks, share, p, q);
+    sm[0][ty][tx] = p;
+    sm[1][ty][tx] = q;
+    __syncthreads();
+    if (j == 0 && g < A.groups) {
+      for (int k = 1; k < share; ++k) {
+        p += sm[0][ty + k][tx];
+        q += sm[1][ty + k][tx];
       }
-      __syncthreads();
+      close_group(g, p, q);
     }
+    __syncthreads();
   }
   sm[0][ty][tx] = P;
   sm[1][ty][tx] = Q;

@@ -148,48 +148,53 @@ __device__ __forceinline__ void sum_over(float (&v)[N], const TeamCtx& t, TeamSu
 
 template <int V>
 __device__ __forceinline__ float sum8(const float (&f)[V][8]) {
-  float s = 0.f;
+  float2 s = both(0.f);
 #pragma unroll
   for (int v = 0; v < V; ++v)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s += f[v][k];
-  return s;
+    for (int k = 0; k < 4; ++k) s = __fadd2_rn(s, pair(f[v], k));
+  return s.x + s.y;
 }
 template <int V>
 __device__ __forceinline__ float dot8(const float (&f)[V][8], const float (&g)[V][8]) {
-  float s = 0.f;
+  float2 s = both(0.f);
 #pragma unroll
   for (int v = 0; v < V; ++v)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s = fmaf(f[v][k], g[v][k], s);
-  return s;
+    for (int k = 0; k < 4; ++k) s = __ffma2_rn(pair(f[v], k), pair(g[v], k), s);
+  return s.x + s.y;
 }
-// Takes a mean off; places behind the last feature (n[v] of a vector are
-// before it) stay 0.
-template <int V>
+// Zeros at and behind element n of a vector (kVec: n is 0 or 8).
+template <bool kVec>
+__device__ __forceinline__ void clear_behind(float (&f)[8], int n) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] = (kVec ? n > 0 : k < n) ? f[k] : 0.f;
+}
+// Takes a mean off; places behind the last feature stay 0.
+template <int V, bool kVec>
 __device__ __forceinline__ void centre(float (&f)[V][8], float mean, const int (&n)[V]) {
 #pragma unroll
-  for (int v = 0; v < V; ++v)
+  for (int v = 0; v < V; ++v) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[v][k] = k < n[v] ? f[v][k] - mean : 0.f;
+    for (int k = 0; k < 4; ++k) put_pair(f[v], k, __fadd2_rn(pair(f[v], k), both(-mean)));
+    clear_behind<kVec>(f[v], n[v]);
+  }
 }
 template <int V>
 __device__ __forceinline__ void times(float (&f)[V][8], float r) {
 #pragma unroll
-  for (int v = 0; v < V; ++v)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[v][k] *= r;
+  for (int v = 0; v < V; ++v) mul8(f[v], both(r));
 }
 __device__ __forceinline__ float factor(float sum_sq, const Common& c) { return rsqrtf(fmaf(sum_sq, c.inv_d, c.eps)); }
 // Normalises a row in place.  The variance is taken around the mean, a second
 // pass over the registers, so a large mean costs no digits.
-template <int V, bool kLayer>
+template <int V, bool kLayer, bool kVec>
 __device__ __forceinline__ void normalise_row(float (&f)[V][8], const int (&n)[V], const Common& c, const TeamCtx& t,
                                               TeamSums& s, int& turn) {
   if (kLayer) {
     float m[1] = {sum8<V>(f)};
     sum_over(m, t, s, turn);
-    centre<V>(f, m[0] * c.inv_d, n);
+    centre<V, kVec>(f, m[0] * c.inv_d, n);
   }
   float q[1] = {dot8<V>(f, f)};
   sum_over(q, t, s, turn);
@@ -296,19 +301,24 @@ __global__ void __launch_bounds__(kTypedThreads, 1)
 #pragma unroll
         for (int v = 0; v < V; ++v) save_raw<BT>(A.sb, c, step0[v], row, col[v], rb[v], b[v]);
       }
-      if (c.post_norm) normalise_row<V, kLayer>(b, n, c, t, sums, turn);
+      if (c.post_norm) normalise_row<V, kLayer, kVec>(b, n, c, t, sums, turn);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         if (fixed) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            x[v][k] = fmaf(b[v][k], mul[v][k], kLayer ? x[v][k] + add[kLayer ? v : 0][k] : x[v][k]);
+          for (int k = 0; k < 4; ++k) {
+            const float2 y = kLayer ? __fadd2_rn(pair(x[v], k), pair(add[kLayer ? v : 0], k)) : pair(x[v], k);
+            put_pair(x[v], k, __ffma2_rn(pair(b[v], k), pair(mul[v], k), y));
+          }
         } else {
           float g[8];
           gate8(c, row, col[v], g);
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            x[v][k] = fmaf(kLayer ? fmaf(b[v][k], mul[v][k], add[kLayer ? v : 0][k]) : b[v][k] * mul[v][k], g[k], x[v][k]);
+          for (int k = 0; k < 4; ++k) {
+            const float2 y = kLayer ? __ffma2_rn(pair(b[v], k), pair(mul[v], k), pair(add[kLayer ? v : 0], k))
+                                    : __fmul2_rn(pair(b[v], k), pair(mul[v], k));
+            put_pair(x[v], k, __ffma2_rn(y, pair(g, k), pair(x[v], k)));
+          }
         }
         rx[v] = pack<XT>(x[v]);
         if (n[v]) store_part<XT, kVec>(A.x_out, at(row, A.x_out.ld, col[v]), n[v], rx[v]);
@@ -323,11 +333,13 @@ __global__ void __launch_bounds__(kTypedThreads, 1)
       }
     }
     if (!has_y) continue;
-    normalise_row<V, kLayer>(x, n, c, t, sums, turn);
+    normalise_row<V, kLayer, kVec>(x, n, c, t, sums, turn);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[v][k] = kLayer ? fmaf(x[v][k], pw[v][k], pb[kLayer ? v : 0][k]) : x[v][k] * pw[v][k];
+      for (int k = 0; k < 4; ++k)
+        put_pair(x[v], k, kLayer ? __ffma2_rn(pair(x[v], k), pair(pw[v], k), pair(pb[kLayer ? v : 0], k))
+                                 : __fmul2_rn(pair(x[v], k), pair(pw[v], k)));
       const Raw8<BT> raw = pack<BT>(x[v]);
       if (n[v]) store_part<BT, kVec>(A.y, at(row, A.y.ld, col[v]), n[v], raw);
       if (kSave && A.sy.codes) {
@@ -358,9 +370,7 @@ struct Held<DT, true, kVec> {
   __device__ __forceinline__ void values(const Saved8& s, float (&f)[8]) const {
     decode4(codes.x, s.format, f);
     decode4(codes.y, s.format, f + 4);
-    const float st = step_value(step);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] *= st;
+    mul8(f, both(step_value(step)));
   }
 };
 
@@ -450,15 +460,15 @@ __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __gri
       if (kLayer) {
         float m[2] = {sum8<V>(x), sum8<V>(b)};
         sum_over(m, t, sums, turn);
-        centre<V>(x, m[0] * c.inv_d, n);
-        if (c.post_norm) centre<V>(b, m[1] * c.inv_d, n);
+        centre<V, kVec>(x, m[0] * c.inv_d, n);
+        if (c.post_norm) centre<V, kVec>(b, m[1] * c.inv_d, n);
       }
       {
         float gw[V][8];
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) gw[v][k] = g[v][k] * pw[v][k];
+          for (int k = 0; k < 4; ++k) put_pair(gw[v], k, __fmul2_rn(pair(g[v], k), pair(pw[v], k)));
         float s[4] = {dot8<V>(x, x), dot8<V>(gw, x), dot8<V>(b, b), kLayer ? sum8<V>(gw) : 0.f};
         sum_over(s, t, sums, turn);
         sxx = s[0];
@@ -469,15 +479,17 @@ __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __gri
           const float r = factor(sxx, c);
           const float mgn = sgx * r * c.inv_d, mg = kLayer ? sg * c.inv_d : 0.f;
 #pragma unroll
-          for (int v = 0; v < V; ++v)
+          for (int v = 0; v < V; ++v) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float nk = x[v][k] * r;
-              acc[1][v][k] = fmaf(g[v][k], nk, acc[1][v][k]);
-              if (kLayer) acc[kSums - 1][v][k] += g[v][k];
-              e[v][k] = fmaf(r, fmaf(-nk, mgn, kLayer ? gw[v][k] - mg : gw[v][k]), e[v][k]);
-              if (kLayer && k >= n[v]) e[v][k] = 0.f;
+            for (int k = 0; k < 4; ++k) {
+              const float2 nk = __fmul2_rn(pair(x[v], k), both(r));
+              put_pair(acc[1][v], k, __ffma2_rn(pair(g[v], k), nk, pair(acc[1][v], k)));
+              if (kLayer) put_pair(acc[kSums - 1][v], k, __fadd2_rn(pair(acc[kSums - 1][v], k), pair(g[v], k)));
+              const float2 t0 = kLayer ? __fadd2_rn(pair(gw[v], k), both(-mg)) : pair(gw[v], k);
+              put_pair(e[v], k, __ffma2_rn(both(r), __ffma2_rn(nk, both(-mgn), t0), pair(e[v], k)));
             }
+            if (kLayer) clear_behind<kVec>(e[v], n[v]);
+          }
         }
       }
 #pragma unroll
@@ -522,10 +534,10 @@ __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __gri
 #pragma unroll
       for (int v = 0; v < V; ++v)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          acc[0][v][k] = fmaf(e[v][k], b[v][k], acc[0][v][k]);
-          if (kLayer) acc[kLayer ? 2 : 0][v][k] += e[v][k];
-          e[v][k] *= mul[v][k];
+        for (int k = 0; k < 4; ++k) {
+          put_pair(acc[0][v], k, __ffma2_rn(pair(e[v], k), pair(b[v], k), pair(acc[0][v], k)));
+          if (kLayer) put_pair(acc[kLayer ? 2 : 0][v], k, __fadd2_rn(pair(acc[kLayer ? 2 : 0][v], k), pair(e[v], k)));
+          put_pair(e[v], k, __fmul2_rn(pair(e[v], k), pair(mul[v], k)));
         }
       if (c.post_norm) {
         float mhm, mh = 0.f;
@@ -542,7 +554,10 @@ __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __gri
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) e[v][k] = rb * fmaf(-b[v][k], mhm, kLayer ? e[v][k] - mh : e[v][k]);
+          for (int k = 0; k < 4; ++k) {
+            const float2 t0 = kLayer ? __fadd2_rn(pair(e[v], k), both(-mh)) : pair(e[v], k);
+            put_pair(e[v], k, __fmul2_rn(both(rb), __ffma2_rn(pair(b[v], k), both(-mhm), t0)));
+          }
       }
 #pragma unroll
       for (int v = 0; v < V; ++v)
