@@ -244,8 +244,9 @@ def weight_gradient(saved: SavedActivation, grad_output: torch.Tensor, *, initia
 
     The sum is held in float32.  The saved values enter the tensor cores
     exactly, and so does a bfloat16 gradient; a float16 or float32 gradient is
-    split into two or three bfloat16 terms that add up to it, at two or three
-    times the work.  Equal operands give equal bits."""
+    split into two or three bfloat16 terms that add up to it (but for parts
+    below 2^-133), at two or three times the work.  Equal operands give equal
+    bits.  While it runs, the call holds the activation once in bfloat16."""
     _require_saved(saved, "saved")
     require_cuda(grad_output, "grad_output")
     try:
@@ -328,7 +329,7 @@ def swiglu_backward(grad_h: torch.Tensor, saved_gate: SavedActivation, saved_up:
     float32 and saved, for the weight gradient of the product that reads it --
     so the forward pass need not keep it: ``(grad_gate, grad_up, saved_h)``.
     ``grad_gate`` / ``grad_up``: arrays to write to (row-strided: the halves
-    of a fused projection's gradient)."""
+    of a fused projection's gradient); one of them may be ``grad_h`` itself."""
     require_cuda(grad_h, "grad_h")
     _require_saved(saved_gate, "saved_gate")
     _require_saved(saved_up, "saved_up")
@@ -342,6 +343,8 @@ def swiglu_backward(grad_h: torch.Tensor, saved_gate: SavedActivation, saved_up:
     for name, t in (("grad_gate", grad_gate), ("grad_up", grad_up)):
         if t is not None and (tuple(t.shape) != shape or t.dtype != grad_h.dtype):
             raise ValueError(f"{name} must have grad_h's shape {shape} and dtype {grad_h.dtype}")
+    if grad_gate is not None and grad_up is not None and grad_gate.numel() and grad_gate.data_ptr() == grad_up.data_ptr():
+        raise ValueError("grad_gate and grad_up must be two arrays")
     lib = _lib.load()
     with on_device(device):
         if grad_gate is None:

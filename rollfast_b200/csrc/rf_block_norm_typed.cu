@@ -281,9 +281,14 @@ __global__ void __launch_bounds__(kTypedThreads, 1)
       nb[v] = load_part<BT, kVec>(A.b, at(r, A.b.ld, col[v]), live && has_b ? n[v] : 0);
     }
   };
-  fetch();
+  // Float32 branches, and LayerNorm that saves, have no registers for the next
+  // row: with it, 65536 x 768 saved took 281 instead of 240 us, and LayerNorm
+  // 16384 x 4096 in float32 took 279 instead of 238 us.
+  constexpr bool kAhead = BT != RF_F32 && !(kLayer && kSave);
+  if (kAhead) fetch();
   while (next < rows) {
     const int row = int(next);
+    if (!kAhead) fetch();
     Raw8<XT> rx[V];
     Raw8<BT> rb[V];
     float x[V][8], b[V][8];
@@ -295,7 +300,7 @@ __global__ void __launch_bounds__(kTypedThreads, 1)
       unpack<BT>(rb[v], b[v]);
     }
     next += step;
-    fetch();
+    if (kAhead) fetch();
     if (has_b) {
       if (kSave && A.sb.codes) {
 #pragma unroll
@@ -377,7 +382,9 @@ struct Held<DT, true, kVec> {
 template <int XT, int BT, int V, bool kLayer, bool kSaved, bool kVec>
 __global__ void __launch_bounds__(kTypedThreads, 1) k_norm_bwd_typed(const __grid_constant__ BwdArgs A, int team_threads) {
   constexpr int kSums = kLayer ? 4 : 2;  // P, R, then Q, U
-  constexpr bool kAhead = V == 1;        // wider rows have no registers for the next one
+  // Wider rows and float32 branches have no registers for the next row: with it,
+  // LayerNorm 16384 x 4096 in float32 took 486 instead of 394 us.
+  constexpr bool kAhead = V == 1 && BT != RF_F32;
   __shared__ TeamSums sums;
   extern __shared__ float join[];        // [kSums][team_threads * 8 V] when a CTA has several teams
   int turn = 0;

@@ -340,3 +340,35 @@ def test_no_device_side_wait_gave_up():
 
     torch.cuda.synchronize()
     _lib.sync_check(torch.cuda.current_stream().cuda_stream)
+
+
+def test_swiglu_of_two_formats_and_shared_gradients():
+    import rollfast_b200 as rf
+
+    g, u, d = (_make((33, 264), "bfloat16", s) for s in (20, 21, 22))
+    sg, su = rf.save_activation(g, "int8"), rf.save_activation(u, "e4m3")
+    dg, du, sh = rf.swiglu_backward(d, sg, su, save_h="int8")
+    vg, vu = rf.load_activation(sg), rf.load_activation(su)
+    wg, wu = T.swiglu_grads(_np(d), _np(vg), _np(vu))
+    assert np.allclose(_np(dg), wg, rtol=2.0 ** -7, atol=1e-5) and np.allclose(_np(du), wu, rtol=2.0 ** -7, atol=1e-5)
+    with pytest.raises(ValueError):
+        rf.swiglu_backward(d, sg, su, grad_gate=dg, grad_up=dg)
+    # In place over the incoming gradient.
+    e = d.clone()
+    got = rf.swiglu_backward(e, sg, su, grad_gate=e)
+    assert got[0] is e and torch.equal(e, dg) and torch.equal(got[1], du)
+
+
+def test_weight_gradient_of_many_shapes_on_whole_numbers():
+    """Tiles whole and in parts, one and several waves of them, odd edges."""
+    import rollfast_b200 as rf
+
+    rng = np.random.default_rng(23)
+    for rows, k, n in [(2050, 768, 300), (129, 2600, 2050), (4097, 30, 5000), (300, 5000, 2304), (10000, 257, 257)]:
+        x = torch.from_numpy(rng.integers(-3, 4, (rows, k)).astype(np.float32)).cuda()
+        x[:, ::32] = 127.0
+        g = torch.from_numpy(rng.integers(-2, 3, (rows, n)).astype(np.float32)).cuda().bfloat16()
+        saved = rf.save_activation(x.bfloat16())
+        want = (rf.load_activation(saved, dtype=torch.float32).double().t() @ g.double()).float()
+        assert torch.equal(rf.weight_gradient(saved, g), want)
+        assert torch.equal(rf.weight_gradient(saved, g, layout="oi"), want.t())

@@ -312,3 +312,54 @@ def test_captured_backward_follows_its_inputs():
     want = rf.block_norm_backward(dx, dy, x, b, **kw, **akw, **p)
     for u, v in zip(r, want):
         assert u is None or torch.equal(u, v)
+
+
+@pytest.mark.parametrize("dt", list(TORCH))
+def test_rms_with_biases(dt):
+    shape = (2, 9, 264)
+    x, b, p, kw, akw = _setup(shape, dt, "rms", True, "sequence", "tanh", "vector")
+    p["pre_bias"], p["post_bias"] = _make((264,), "float32", 40, 0.2), _make((264,), "float32", 41, 0.2)
+    _check_forward(x, b, p, kw, akw, save="e4m3")
+    _check_backward(x, b, p, kw, akw, _make(shape, dt, 10, 0.3), _make(shape, dt, 11, 0.3))
+
+
+def test_saved_and_unsaved_inputs_mix():
+    """Either input saved, in either format, gives what its values give."""
+    import rollfast_b200 as rf
+
+    shape = (2, 30, 520)
+    x, b, p, kw, akw = _setup(shape, "float32", "layer", True, "channel", None, "vector")
+    dx, dy = _make(shape, "float32", 10), _make(shape, "float32", 11)
+    sx, sb = rf.save_activation(x, "int8"), rf.save_activation(b, "e4m3")
+    vx, vb = rf.load_activation(sx), rf.load_activation(sb)
+    want = rf.block_norm_backward(dx, dy, vx, vb, **kw, **akw, **p)
+    for pair in ((sx, sb), (sx, vb), (vx, sb)):
+        got = rf.block_norm_backward(dx, dy, *pair, **kw, **akw, **p)
+        for u, v in zip(got, want):
+            assert torch.allclose(u, v, rtol=1e-4, atol=1e-5)
+    only = rf.block_norm_backward(dx, None, sx, sb, **kw, **akw, **p)
+    assert torch.equal(only.x, dx) and (only.pre_weight == 0).all()
+
+
+def test_many_short_sequences():
+    """More gate groups than the GPU holds at once, of two rows each."""
+    shape = (3000, 2, 72)
+    x, b, p, kw, akw = _setup(shape, "float32", "rms", True, "sequence", None, "one")
+    _check_forward(x, b, p, kw, akw)
+    _check_backward(x, b, p, kw, akw, _make(shape, "float32", 10, 0.3), _make(shape, "float32", 11, 0.3))
+
+
+def test_rows_past_32_bit_offsets():
+    import rollfast_b200 as rf
+
+    rows, d = 300_001, 7_168  # 2.15e9 elements
+    x = torch.zeros(rows, d, dtype=torch.bfloat16, device="cuda")
+    x[-1] = _make((d,), "bfloat16", 50, 2.0)
+    y = rf.block_norm_forward(x, eps=1e-6).y
+    assert torch.equal(y[-1], rf.block_norm_forward(x[-1:].clone(), eps=1e-6).y[0])
+    assert int((y[:-1] != 0).sum()) == 0
+    g = torch.zeros_like(x)
+    g[-1] = 1.0
+    r = rf.block_norm_backward(None, g, x, eps=1e-6, pre_weight=torch.ones(d, device="cuda"))
+    one = rf.block_norm_backward(None, g[-1:].clone(), x[-1:].clone(), eps=1e-6, pre_weight=torch.ones(d, device="cuda"))
+    assert torch.equal(r.x[-1], one.x[0]) and torch.allclose(r.pre_weight, one.pre_weight, rtol=1e-6)
