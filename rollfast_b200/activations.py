@@ -64,8 +64,7 @@ class SavedActivation:
         self.rows, self.features = rows, features = _rows_features(shape, "a saved activation")
         self.shape, self.dtype, self.format = shape, dtype, format
         self._codes = self._scales = None
-        self._buffer = torch.empty(_up(rows * _up(features, 16), 256) + -(-features // 128) * _up(rows, 64) * 4,
-                                   dtype=torch.uint8, device=device)
+        self._buffer = fresh_bytes(_up(rows * _up(features, 16), 256) + -(-features // 128) * _up(rows, 64) * 4, device)
         return self
 
     @property
@@ -159,13 +158,24 @@ _here = contextlib.nullcontext()
 def on_device(device: torch.device):
     """A launch must come from the arrays' device; switching costs more than
     the check that it is current already."""
-    return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _here if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def stream_of(device: torch.device) -> int:
     """Handle of the current stream, without a Stream object: that takes
     microseconds, as much as a small call's launch."""
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def fresh(like: torch.Tensor) -> torch.Tensor:
+    """A contiguous array of ``like``'s shape and type, by the quickest way
+    that makes one: of a small call's time, half went into ``torch.empty``."""
+    return torch.empty_like(like) if like.is_contiguous() else torch.empty(like.shape, dtype=like.dtype,
+                                                                           device=like.device)
+
+
+def fresh_bytes(n: int, device: torch.device) -> torch.Tensor:
+    return torch.empty_strided((n,), (1,), dtype=torch.uint8, device=device)
 
 
 def require_same_device(device: torch.device, **tensors) -> None:
@@ -286,7 +296,7 @@ def weight_gradient(saved: SavedActivation, grad_output: torch.Tensor, *, initia
                                                          gdt, ctypes.byref(nbytes)))
         # Allocated per call: a cached buffer would be shared by CUDA graphs
         # that are captured on one stream and replayed on two.
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device) if nbytes.value else None
+        ws = fresh_bytes(nbytes.value, device) if nbytes.value else None
         _lib.check(lib.rf_weight_gradient(native(saved), grad_output.data_ptr(), ldg, gdt, n_out, code,
                                           None if initial is None else initial.data_ptr(), out.data_ptr(), ld_out,
                                           rf_dtype(out), None if ws is None else ws.data_ptr(), nbytes.value,
@@ -309,7 +319,7 @@ def swiglu_forward(gate: torch.Tensor, up: torch.Tensor, format: str | None = "i
     device = gate.device
     lib = _lib.load()
     with on_device(device):
-        h = torch.empty(gate.shape, dtype=gate.dtype, device=device)
+        h = fresh(gate)
         sg = su = None
         if format is not None:
             sg = empty_saved(gate.shape, gate.dtype, format, device)
@@ -348,9 +358,9 @@ def swiglu_backward(grad_h: torch.Tensor, saved_gate: SavedActivation, saved_up:
     lib = _lib.load()
     with on_device(device):
         if grad_gate is None:
-            grad_gate = torch.empty(shape, dtype=grad_h.dtype, device=device)
+            grad_gate = fresh(grad_h)
         if grad_up is None:
-            grad_up = torch.empty(shape, dtype=grad_h.dtype, device=device)
+            grad_up = fresh(grad_h)
         ldg, ldu = _out_rows(grad_gate, "grad_gate"), _out_rows(grad_up, "grad_up")
         saved_h = None if save_h is None else empty_saved(shape, saved_gate.dtype, save_h, device)
         grad_h, ldh = row_strided(grad_h)

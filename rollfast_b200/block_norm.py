@@ -25,8 +25,8 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .activations import (SavedActivation, _format_code, _require_saved, _rows_features, empty_saved, native,
-                          on_device, require_same_device, row_strided, stream_of)
+from .activations import (SavedActivation, _format_code, _require_saved, _rows_features, empty_saved, fresh,
+                          fresh_bytes, native, on_device, require_same_device, row_strided, stream_of)
 from .base import require_cuda, rf_dtype
 
 _KINDS = {"rms": _lib.RF_RMS_NORM, "layer": _lib.RF_LAYER_NORM}
@@ -132,6 +132,16 @@ def _rows(t, what: str, shape):
     return _lib.RfRows(t.data_ptr(), ld, dt, None), t
 
 
+def _like(t, others, device):
+    """An array for the gradient of ``t``, a tensor or a saved activation."""
+    if isinstance(t, torch.Tensor):
+        return fresh(t)
+    for o in others:  # of the same shape
+        if o is not None and o.dtype == t.dtype:
+            return fresh(o)
+    return torch.empty(t.shape, dtype=t.dtype, device=device)
+
+
 def block_norm_forward(x: torch.Tensor, branch: torch.Tensor | None = None, *, kind: str = "rms", eps: float = 1e-6,
                        post_norm: bool = True, pre_norm: bool = True, pre_weight: torch.Tensor | None = None,
                        pre_bias: torch.Tensor | None = None, post_weight: torch.Tensor | None = None,
@@ -163,8 +173,8 @@ def block_norm_forward(x: torch.Tensor, branch: torch.Tensor | None = None, *, k
     with on_device(device):
         cx, alive_x = _rows(x, "x", shape)
         cb, alive_b = (None, None) if branch is None else _rows(branch, "branch", shape)
-        out = torch.empty(shape, dtype=x.dtype, device=device) if branch is not None else x
-        y = torch.empty(shape, dtype=x.dtype if branch is None else branch.dtype, device=device) if pre_norm else None
+        out = fresh(x) if branch is not None else x
+        y = fresh(x if branch is None else branch) if pre_norm else None
         saved = [None if save is None or t is None else empty_saved(shape, t.dtype, save, device)
                  for t in (out, branch, y)]
         co = None if branch is None else _rows(out, "x", shape)[0]
@@ -215,10 +225,10 @@ def block_norm_backward(grad_x: torch.Tensor | None, grad_y: torch.Tensor | None
             args.append(c)
             alive.append(a)
         empty = p.rows == 0
-        make = torch.zeros if empty else torch.empty
-        out_x = torch.empty(shape, dtype=x.dtype, device=device)
-        out_b = None if branch is None else torch.empty(shape, dtype=branch.dtype, device=device)
-        grads = {n: make(t.shape, dtype=t.dtype, device=device) for n, t in keep.items()}
+        make = torch.zeros_like if empty else torch.empty_like
+        out_x = _like(x, (grad_x, grad_y), device)
+        out_b = None if branch is None else _like(branch, (grad_y, grad_x), device)
+        grads = {n: make(t) for n, t in keep.items()}
         if not empty:
             for n, t in grads.items():
                 getattr(p, n).grad = t.data_ptr()
@@ -226,7 +236,7 @@ def block_norm_backward(grad_x: torch.Tensor | None, grad_y: torch.Tensor | None
             args.append(None if out_b is None else _rows(out_b, "branch", shape)[0])
             nbytes = ctypes.c_size_t()
             _lib.check(lib.rf_block_norm_workspace_size(p, ctypes.byref(nbytes)))
-            ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device) if nbytes.value else None
+            ws = fresh_bytes(nbytes.value, device) if nbytes.value else None
             _lib.check(lib.rf_block_norm_backward(p, *args, None if ws is None else ws.data_ptr(), nbytes.value,
                                                   stream_of(device)))
     del alive
