@@ -10,10 +10,11 @@
 // loads in flight; others (odd widths, shifted views) through one of the
 // simple kernels below them.
 // Measured on a B200, bfloat16, int8 (a copy: 6549 GB/s): 16384 x 14336 saved
-// in 117 us (6.1 TB/s), loaded in 117, saved stochastically in 217 (e4m3 236;
-// there the generator's integer work is the bound, 28 instructions an
-// element); SwiGLU 8192 x 14336 forward 164 us (5.8 TB/s), backward 170, with
-// h saved 199 (5.4).
+// in 117 us (6.1 TB/s), loaded in 117, saved stochastically in 219 in either
+// format (there the generator's integer work is the bound, 28 instructions an
+// element; e4m3 took 238 while values below its normal range were looked for
+// element by element after the scaling, not two at a time before it); SwiGLU
+// 8192 x 14336 forward 165 us (5.7 TB/s), backward 172, with h saved 190.
 #include "rf_act8.cuh"
 
 #include <algorithm>
@@ -144,18 +145,20 @@ __device__ __forceinline__ uint2 encode8_stochastic_int8(const float (&f)[8], ui
 // 2^-6 up the noise goes in below the 3 significand bits that stay, and the
 // rest is cut off: the same, since magnitude / step + u has at most 24
 // significant bits below 16, and above 16 only its floor counts.
-__device__ __forceinline__ uint2 encode8_stochastic_e4m3(const float (&f)[8], uint64_t na, uint64_t nb, uint32_t s) {
+// `low`: some magnitude may lie below 2^-6 (and above 0).
+__device__ __forceinline__ uint2 encode8_stochastic_e4m3(const float (&f)[8], uint64_t na, uint64_t nb, uint32_t s,
+                                                         bool low) {
   const float inv = __uint_as_float((254u - s) << 23);
   float g[8];
-  uint32_t least = 0xFFFFFFFFu;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const uint32_t w = noise_word(na, nb, k >> 1);
-    const uint32_t v = __float_as_uint(f[k] * inv);
-    least = min(least, (v & 0x7FFFFFFFu) - 1u);  // 0 wraps around: it rounds to itself either way
-    g[k] = __uint_as_float((v + ((k & 1) ? (w >> 12) & 0xFFFF0u : (w << 4) & 0xFFFF0u)) & 0xFFF00000u);
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t w = noise_word(na, nb, k);
+    const float2 v = __fmul2_rn(pair(f, k), both(inv));
+    // The halves by byte permutation, so that shift and addition are one instruction.
+    g[2 * k] = __uint_as_float((__float_as_uint(v.x) + (__byte_perm(w, 0u, 0x4410) << 4)) & 0xFFF00000u);
+    g[2 * k + 1] = __uint_as_float((__float_as_uint(v.y) + (__byte_perm(w, 0u, 0x4432) << 4)) & 0xFFF00000u);
   }
-  if (least < 0x3C800000u - 1u) {  // some magnitude is below 2^-6
+  if (low) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const float v = f[k] * inv, m = fabsf(v);
@@ -166,10 +169,30 @@ __device__ __forceinline__ uint2 encode8_stochastic_e4m3(const float (&f)[8], ui
   }
   return encode8(g, 127u, RF_E4M3);  // step 1: the values are on the grid, or above 448 and saturate
 }
+// Whether a vector holds a magnitude in (0, 2^-6) steps, for the e4m3 code.
+__device__ __forceinline__ bool any_low(const float (&f)[8], uint32_t s) {
+  uint32_t least = 0xFFFFFFFFu;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) least = min(least, (__float_as_uint(f[k]) & 0x7FFFFFFFu) - 1u);  // 0 wraps around
+  return s <= 6u || least < ((s - 6u) << 23) - 1u;
+}
+// The same of bfloat16 as it lies in memory, two at a time.  Where the low
+// half is 0, the subtraction takes one more from the high half: a magnitude of
+// 2^-133 may go unseen, which every draw rounds to 0 from steps of 2^-107 up
+// (smaller steps count as low), and one more may be seen, which only takes the
+// longer path.
+template <int DT>
+__device__ __forceinline__ bool any_low(const Raw8<DT>& r, const float (&f)[8], uint32_t s) {
+  if (DT != RF_BF16) return any_low(f, s);
+  const uint32_t a = __vminu2((r.u[0].x & 0x7FFF7FFFu) - 0x00010001u, (r.u[0].y & 0x7FFF7FFFu) - 0x00010001u);
+  const uint32_t b = __vminu2((r.u[0].z & 0x7FFF7FFFu) - 0x00010001u, (r.u[0].w & 0x7FFF7FFFu) - 0x00010001u);
+  const uint32_t m = __vminu2(a, b);
+  return s <= 20u || min(m & 0xFFFFu, m >> 16) < ((s - 6u) << 7) - 1u;
+}
 __device__ __forceinline__ uint2 encode8_stochastic(const float (&f)[8], uint64_t a, uint64_t b, uint32_t s,
-                                                    int format) {
+                                                    int format, bool low) {
   if (s == kNanStep) return make_uint2(0u, 0u);
-  return format == RF_INT8 ? encode8_stochastic_int8(f, a, b, s) : encode8_stochastic_e4m3(f, a, b, s);
+  return format == RF_INT8 ? encode8_stochastic_int8(f, a, b, s) : encode8_stochastic_e4m3(f, a, b, s, low);
 }
 
 // One thread's column of an array, walked down by rows.  Addresses move by
@@ -255,7 +278,8 @@ __global__ void __launch_bounds__(kThreads) k_save_typed(const void* x, int64_t 
       unpack<DT>(cur[r], f);
       uint2 c;
       if (kStochastic) {
-        c = encode8_stochastic(f, splitmix64_mix(z), splitmix64_mix(z + kSplitmixGamma), s, kFormat);
+        c = encode8_stochastic(f, splitmix64_mix(z), splitmix64_mix(z + kSplitmixGamma), s, kFormat,
+                               kFormat == RF_E4M3 && any_low<DT>(cur[r], f, s));
         z += row_state;
       } else {
         c = encode8(f, s, kFormat);
@@ -351,7 +375,7 @@ __global__ void __launch_bounds__(kThreads) k_save(RowView x, Saved8 out, int64_
     if (kStochastic) {
       uint64_t na, nb;
       noise8(seed, uint64_t(row) * uint64_t(features) + uint64_t(col), na, nb);
-      c = encode8_stochastic(f[r], na, nb, s, out.format);
+      c = encode8_stochastic(f[r], na, nb, s, out.format, any_low(f[r], s));
     } else {
       c = encode8(f[r], s, out.format);
     }

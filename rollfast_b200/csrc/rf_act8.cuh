@@ -13,8 +13,9 @@
 //
 // Codes: [rows][ld] bytes, ld = features rounded up to 16, zeros behind the
 // last feature.  Steps: [panels of 128 features][scale_rows][4], scale_rows =
-// rows rounded up to 64, so that the steps of a 64 x 128 tile are 256
-// contiguous bytes; blocks behind the last feature hold 1.
+// rows rounded up to 64: a warp that reads 128 features of consecutive rows
+// reads consecutive words, and panels start on 256-byte boundaries; blocks
+// behind the last feature hold 1.
 #pragma once
 
 #include <cuda_fp8.h>

@@ -3,6 +3,10 @@
 //
 //   x' = x + s a(gamma) N_post(b),   y = N_pre(x')
 //
+// The C entry points and the kernels for every type and width; the usual
+// types up to 8192 features go through rf_block_norm_typed.cu's kernels, which
+// hold their rows the same way and are 2 to 3 times as fast.
+//
 // Both directions are bound by HBM: a row is read once, held in registers
 // while its statistics are formed, and each output is written once.  A row
 // belongs to a team: one warp up to 1024 features (no barrier), else the

@@ -126,9 +126,9 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // The same without a release at cluster scope, which waits until all earlier
-// writes of the thread are visible to the whole cluster (about a microsecond):
-// for writes to this CTA's own shared memory that a proxy fence has completed
-// already and that only the tensor core of this SM reads.
+// writes of the thread are visible to the whole cluster (about a microsecond).
+// It hands over no memory: a caller signals that its reads of TMEM are done
+// (tcgen05.wait::ld and the fence before it).
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -158,19 +158,6 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
       : "memory");
 }
 
-// Untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned).
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bar, uint32_t bytes) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
-               : "memory");
-}
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
-      : "memory");
-}
 // Whether a phase is complete, without waiting: issued ahead of other work, its
 // latency (about 200 cycles) passes behind it.
 __device__ __forceinline__ uint32_t mbar_test(uint32_t bar, uint32_t parity) {

@@ -94,6 +94,24 @@ def test_special_values(fmt, seed):
     assert (half[4] == 65504).all() and half[1].isnan().sum() == 32
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dt", ["bfloat16", "float32"])
+@pytest.mark.parametrize("features", [256, 250])
+@pytest.mark.parametrize("seed", [None, 7])
+def test_wide_and_tiny_ranges_within_a_block(fmt, dt, features, seed):
+    """Magnitudes from the type's least to the block's largest, at largest
+    values of 2^-130 to 2^-1: below a step, subnormal in the code, and zeros."""
+    import rollfast_b200 as rf
+
+    rng = np.random.default_rng(11)
+    top = -130 + np.arange(130)[:, None]
+    low = np.maximum(top - 18, -133)
+    e = low + np.floor(rng.random((130, features)) * (top - low + 1))
+    v = np.ldexp(rng.choice([-1.0, 1.0], e.shape), e.astype(int)) * (rng.random(e.shape) > 0.1)
+    x = torch.from_numpy(v).to(torch.float32).cuda().to(TORCH[dt])
+    _codes_equal(rf.save_activation(x, fmt, seed=seed), x, seed)
+
+
 def test_row_strided_views_are_read_in_place():
     import rollfast_b200 as rf
 
