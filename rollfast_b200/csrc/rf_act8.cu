@@ -15,6 +15,9 @@
 // element; e4m3 took 238 while values below its normal range were looked for
 // element by element after the scaling, not two at a time before it); SwiGLU
 // 8192 x 14336 forward 165 us (5.7 TB/s), backward 172, with h saved 190.
+// 16384 x 4097, off the boundaries: saved in 76 us (4096: 41), loaded in 92
+// (40), SwiGLU forward 211 (96), backward 243 (102); there a vector takes two
+// or three loads and 13 to 17 selects, and the kernels hold 16 to 24 warps an SM.
 #include "rf_act8.cuh"
 
 #include <algorithm>
@@ -46,6 +49,14 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Threads along a row of nv vectors: a multiple of 16 holds whole panels; whole
+// warps for the shuffles.  Wide rows are cut into equal column tiles, so that
+// few threads of the last one idle (4097 columns: 3 x 192 threads for 528
+// vectors, not 3 x 256: SwiGLU forward 16384 x 4097 in 211 us, not 262).
+int row_threads(int64_t nv) {
+  return int(nv == 16 ? 16 : round_up(ceil_div(nv, ceil_div(nv, int64_t(kThreads))), 32));
+}
+
 // Whole tiles of a typed kernel: CTAs of tx x ty threads over 8-feature
 // vectors x rows, rows_per_thread rows per thread and tile; grid.y column tiles, and
 // along x as many CTAs as the GPU holds, each walking down the rows.
@@ -55,8 +66,7 @@ struct Walk {
 template <auto kernel>
 Walk walk(int64_t rows, int64_t features, int rows_per_thread, int elements = 8) {
   const int64_t nv = ceil_div(features, kPanel8) * (kPanel8 / elements);
-  const int tx = int(nv >= kThreads ? kThreads : nv == 16 ? 16 : round_up(nv, 32));
-  const int ty = kThreads / tx;
+  const int tx = row_threads(nv), ty = kThreads / tx;
   const int64_t gy = ceil_div(nv, tx), tiles = ceil_div(rows, int64_t(ty) * rows_per_thread);
   // Asked once per kernel (and block size: whole warps up to 256 threads): the
   // answer is the same on every GPU of the kind, and asking takes microseconds.
@@ -85,9 +95,7 @@ struct Tiling {
 };
 Tiling tiling(int64_t rows, int64_t features, int rows_per_thread) {
   const int64_t nv = ceil_div(features, kPanel8) * (kPanel8 / 8);
-  // A multiple of 16 threads holds whole panels; whole warps for the shuffles.
-  const int tx = int(nv >= kThreads ? kThreads : nv == 16 ? 16 : round_up(nv, 32));
-  const int ty = kThreads / tx;
+  const int tx = row_threads(nv), ty = kThreads / tx;
   const int64_t gy = ceil_div(rows, int64_t(ty) * rows_per_thread);
   Tiling t;
   t.block = dim3(unsigned(tx), unsigned(ty));
@@ -354,52 +362,56 @@ __global__ void __launch_bounds__(kThreads) k_load_typed(Saved8 in, void* out, i
   }
 }
 
-template <int kRows, bool kStochastic>
+// Neighbouring lanes that hold one row's vectors (tiling).
+__device__ __forceinline__ int row_lanes() { return blockDim.x < 32 ? 16 : 32; }
+
+template <int DT, int kRows, bool kStochastic>
 __global__ void __launch_bounds__(kThreads) k_save(RowView x, Saved8 out, int64_t rows, int64_t features,
                                                    uint64_t seed) {
   const int64_t col = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 8;
   const int64_t row0 = int64_t(blockIdx.x) * blockDim.y * kRows + threadIdx.y;
   const bool in = col < round_up_dev(features, kPanel8);
-  float f[kRows][8];
+  Span8<DT> span[kRows];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int64_t row = row0 + int64_t(r) * blockDim.y;
-    load8(x, row, col, row < rows ? features : 0, f[r]);
+    span[r] = fetch_span<DT>(x, row * x.ld + col, row < rows ? features - col : 0);
   }
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int64_t row = row0 + int64_t(r) * blockDim.y;
-    const uint32_t s = step_byte(block_max_bits(f[r]), out.format);
+    const Raw8<DT> raw = align_span<DT>(span[r], x, row * x.ld + col, row < rows ? features - col : 0);
+    float f[8];
+    unpack<DT>(raw, f);
+    const uint32_t s = step_byte(raw_max_bits<DT>(raw), out.format);
     if (!in || row >= rows) continue;
     uint2 c;
     if (kStochastic) {
       uint64_t na, nb;
       noise8(seed, uint64_t(row) * uint64_t(features) + uint64_t(col), na, nb);
-      c = encode8_stochastic(f[r], na, nb, s, out.format, any_low(f[r], s));
+      c = encode8_stochastic(f, na, nb, s, out.format, out.format == RF_E4M3 && any_low<DT>(raw, f, s));
     } else {
-      c = encode8(f[r], s, out.format);
+      c = encode8(f, s, out.format);
     }
     store_saved(out, row, col, c, s);
   }
 }
 
-template <int kRows>
+template <int DT, int kRows>
 __global__ void __launch_bounds__(kThreads) k_load(Saved8 in, RowOut out, int64_t rows, int64_t features) {
   const int64_t col = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 8;
   const int64_t row0 = int64_t(blockIdx.x) * blockDim.y * kRows + threadIdx.y;
-  if (col >= features) return;
   float f[kRows][8];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int64_t row = row0 + int64_t(r) * blockDim.y;
-    if (row < rows) load8(in, row, col, f[r]);
+    load8(in, row < rows ? row : 0, row < rows ? col : in.ld, f[r]);
   }
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int64_t row = row0 + int64_t(r) * blockDim.y;
-    if (row >= rows) continue;
-    saturate8(out.dt, f[r]);
-    store8(out, row, col, features, f[r]);
+    saturate8(DT, f[r]);
+    store_span<DT>(out.p, row * out.ld + col, row < rows ? features - col : 0, pack<DT>(f[r]), row_lanes());
   }
 }
 
@@ -560,51 +572,54 @@ __global__ void __launch_bounds__(kThreads) k_swiglu_bwd_typed(const void* dh, i
   }
 }
 
-template <int kRows, bool kSave>
+template <int DT, int kRows, bool kSave>
 __global__ void __launch_bounds__(kThreads) k_swiglu_fwd(RowView gate, RowView up, RowOut h, Saved8 sg, Saved8 su,
                                                          int64_t rows, int64_t features) {
   const int64_t col = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 8;
   const int64_t row0 = int64_t(blockIdx.x) * blockDim.y * kRows + threadIdx.y;
   const bool in = col < round_up_dev(features, kPanel8);
-  float g[kRows][8], u[kRows][8];
+  Span8<DT> ng[kRows], nu[kRows];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    const int64_t row = row0 + int64_t(r) * blockDim.y;
-    const int64_t n = row < rows ? features : 0;
-    load8(gate, row, col, n, g[r]);
-    load8(up, row, col, n, u[r]);
+    const int64_t row = row0 + int64_t(r) * blockDim.y, left = row < rows ? features - col : 0;
+    ng[r] = fetch_span<DT>(gate, row * gate.ld + col, left);
+    nu[r] = fetch_span<DT>(up, row * up.ld + col, left);
   }
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    const int64_t row = row0 + int64_t(r) * blockDim.y;
-    const bool live = in && row < rows;
+    const int64_t row = row0 + int64_t(r) * blockDim.y, left = row < rows ? features - col : 0;
+    const Raw8<DT> rg = align_span<DT>(ng[r], gate, row * gate.ld + col, left);
+    const Raw8<DT> ru = align_span<DT>(nu[r], up, row * up.ld + col, left);
+    float g[8], u[8];
+    unpack<DT>(rg, g);
+    unpack<DT>(ru, u);
     if (kSave) {
-      const uint32_t a = step_byte(block_max_bits(g[r]), sg.format);
-      const uint32_t b = step_byte(block_max_bits(u[r]), su.format);
-      if (live) {
-        store_saved(sg, row, col, encode8(g[r], a, sg.format), a);
-        store_saved(su, row, col, encode8(u[r], b, su.format), b);
+      const uint32_t a = step_byte(raw_max_bits<DT>(rg), sg.format);
+      const uint32_t b = step_byte(raw_max_bits<DT>(ru), su.format);
+      if (in && row < rows) {
+        store_saved(sg, row, col, encode8(g, a, sg.format), a);
+        store_saved(su, row, col, encode8(u, b, su.format), b);
       }
     }
-    if (!live) continue;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) g[r][k] = g[r][k] * sigmoid(g[r][k]) * u[r][k];
-    store8(h, row, col, features, g[r]);
+    for (int k = 0; k < 8; ++k) g[k] = g[k] * sigmoid(g[k]) * u[k];
+    store_span<DT>(h.p, row * h.ld + col, left, pack<DT>(g), row_lanes());
   }
 }
 
-template <int kRows, bool kSave>
+template <int DT, int kRows, bool kSave>
 __global__ void __launch_bounds__(kThreads) k_swiglu_bwd(RowView dh, Saved8 gate, Saved8 up, RowOut dgate, RowOut dup,
                                                          Saved8 sh, int64_t rows, int64_t features) {
   const int64_t col = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 8;
   const int64_t row0 = int64_t(blockIdx.x) * blockDim.y * kRows + threadIdx.y;
   const bool in = col < round_up_dev(features, kPanel8);
-  float d[kRows][8], g[kRows][8], u[kRows][8];
+  Span8<DT> nd[kRows];
+  float g[kRows][8], u[kRows][8];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const int64_t row = row0 + int64_t(r) * blockDim.y;
     const bool live = in && row < rows;
-    load8(dh, row, col, live ? features : 0, d[r]);
+    nd[r] = fetch_span<DT>(dh, row * dh.ld + col, live ? features - col : 0);
     load8(gate, live ? row : 0, live ? col : gate.ld, g[r]);
     load8(up, live ? row : 0, live ? col : up.ld, u[r]);
   }
@@ -612,15 +627,16 @@ __global__ void __launch_bounds__(kThreads) k_swiglu_bwd(RowView dh, Saved8 gate
   for (int r = 0; r < kRows; ++r) {
     const int64_t row = row0 + int64_t(r) * blockDim.y;
     const bool live = in && row < rows;
-    float h[8];
-    swiglu_back8(d[r], g[r], u[r], h);
+    const int64_t left = live ? features - col : 0;
+    float d[8], h[8];
+    unpack<DT>(align_span<DT>(nd[r], dh, row * dh.ld + col, left), d);
+    swiglu_back8(d, g[r], u[r], h);
     if (kSave) {
       const uint32_t b = step_byte(block_max_bits(h), sh.format);
       if (live) store_saved(sh, row, col, encode8(h, b, sh.format), b);
     }
-    if (!live) continue;
-    store8(dgate, row, col, features, g[r]);
-    store8(dup, row, col, features, u[r]);
+    store_span<DT>(dgate.p, row * dgate.ld + col, left, pack<DT>(g[r]), row_lanes());
+    store_span<DT>(dup.p, row * dup.ld + col, left, pack<DT>(u[r]), row_lanes());
   }
 }
 
@@ -633,16 +649,19 @@ rf_status check_rows(const void* p, int64_t ld, int32_t dt, int64_t rows, int64_
   return RF_OK;
 }
 
-// Calls f with the element type and the format as constants.
+// Calls f with the element type, or with it and the format, as constants.
+template <typename F>
+void with_type(int32_t dt, F&& f) {
+  if (dt == RF_F32) f(std::integral_constant<int, RF_F32>{});
+  else if (dt == RF_BF16) f(std::integral_constant<int, RF_BF16>{});
+  else f(std::integral_constant<int, RF_F16>{});
+}
 template <typename F>
 void with_types(int32_t dt, int32_t format, F&& f) {
-  auto by_format = [&](auto t) {
+  with_type(dt, [&](auto t) {
     if (format == RF_INT8) f(t, std::integral_constant<int, RF_INT8>{});
     else f(t, std::integral_constant<int, RF_E4M3>{});
-  };
-  if (dt == RF_F32) by_format(std::integral_constant<int, RF_F32>{});
-  else if (dt == RF_BF16) by_format(std::integral_constant<int, RF_BF16>{});
-  else by_format(std::integral_constant<int, RF_F16>{});
+  });
 }
 // Rows of 8-element vectors on 16-byte boundaries.
 bool typed(int64_t features, const void* p, int64_t ld, int32_t dt) {
@@ -676,11 +695,13 @@ extern "C" rf_status rf_save_activation(const void* x, int64_t ldx, int32_t dtyp
     });
     return check_launch("k_save");
   }
-  const Tiling t = tiling(out->rows, out->features, 4);
-  if (stochastic)
-    k_save<4, true><<<t.grid, t.block, 0, st>>>(row_view(x, ldx, dtype), saved8(*out), out->rows, out->features, seed);
-  else
-    k_save<4, false><<<t.grid, t.block, 0, st>>>(row_view(x, ldx, dtype), saved8(*out), out->rows, out->features, 0);
+  const Tiling t = tiling(out->rows, out->features, 2);
+  with_type(dtype, [&](auto dt) {
+    auto go = [&](auto kernel) {
+      kernel<<<t.grid, t.block, 0, st>>>(row_view(x, ldx, dtype, out->rows, out->features), saved8(*out), out->rows, out->features, seed);
+    };
+    stochastic ? go(k_save<decltype(dt)::value, 2, true>) : go(k_save<decltype(dt)::value, 2, false>);
+  });
   return check_launch("k_save");
 }
 
@@ -699,9 +720,11 @@ extern "C" rf_status rf_load_activation(const rf_saved_activation* saved, void* 
     });
     return check_launch("k_load");
   }
-  const Tiling t = tiling(saved->rows, saved->features, 4);
-  k_load<4><<<t.grid, t.block, 0, st>>>(saved8(*saved), row_out(out, ldo, dtype),
-                                                                       saved->rows, saved->features);
+  const Tiling t = tiling(saved->rows, saved->features, 2);
+  with_type(dtype, [&](auto dt) {
+    k_load<decltype(dt)::value, 2>
+        <<<t.grid, t.block, 0, st>>>(saved8(*saved), row_out(out, ldo, dtype), saved->rows, saved->features);
+  });
   return check_launch("k_load");
 }
 
@@ -739,11 +762,13 @@ extern "C" rf_status rf_swiglu_forward(const void* gate, int64_t ld_gate, const 
     });
     return check_launch("k_swiglu_fwd");
   }
-  const Tiling t = tiling(rows, features, 2);
-  const RowView g = row_view(gate, ld_gate, dtype), u = row_view(up, ld_up, dtype);
+  const Tiling t = tiling(rows, features, 1);
+  const RowView g = row_view(gate, ld_gate, dtype, rows, features), u = row_view(up, ld_up, dtype, rows, features);
   const RowOut o = row_out(h, ld_h, dtype);
-  if (saved_gate) k_swiglu_fwd<2, true><<<t.grid, t.block, 0, st>>>(g, u, o, sg, su, rows, features);
-  else k_swiglu_fwd<2, false><<<t.grid, t.block, 0, st>>>(g, u, o, sg, su, rows, features);
+  with_type(dtype, [&](auto dt) {
+    auto go = [&](auto kernel) { kernel<<<t.grid, t.block, 0, st>>>(g, u, o, sg, su, rows, features); };
+    saved_gate ? go(k_swiglu_fwd<decltype(dt)::value, 1, true>) : go(k_swiglu_fwd<decltype(dt)::value, 1, false>);
+  });
   return check_launch("k_swiglu_fwd");
 }
 
@@ -782,14 +807,14 @@ extern "C" rf_status rf_swiglu_backward(const void* grad_h, int64_t ld_grad, con
     });
     return check_launch("k_swiglu_bwd");
   }
-  const Tiling t = tiling(rows, features, 2);
-  const RowView d = row_view(grad_h, ld_grad, dtype);
+  const Tiling t = tiling(rows, features, 1);
+  const RowView d = row_view(grad_h, ld_grad, dtype, rows, features);
   const RowOut dg = row_out(grad_gate, ld_gate, dtype), du = row_out(grad_up, ld_up, dtype);
-  if (saved_h)
-    k_swiglu_bwd<2, true><<<t.grid, t.block, 0, st>>>(d, saved8(*saved_gate), saved8(*saved_up), dg, du, sh, rows,
-                                                      features);
-  else
-    k_swiglu_bwd<2, false><<<t.grid, t.block, 0, st>>>(d, saved8(*saved_gate), saved8(*saved_up), dg, du, sh, rows,
-                                                       features);
+  with_type(dtype, [&](auto dt) {
+    auto go = [&](auto kernel) {
+      kernel<<<t.grid, t.block, 0, st>>>(d, saved8(*saved_gate), saved8(*saved_up), dg, du, sh, rows, features);
+    };
+    saved_h ? go(k_swiglu_bwd<decltype(dt)::value, 1, true>) : go(k_swiglu_bwd<decltype(dt)::value, 1, false>);
+  });
   return check_launch("k_swiglu_bwd");
 }

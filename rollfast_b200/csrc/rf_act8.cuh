@@ -35,6 +35,7 @@ struct RowView {
   int64_t ld;     // elements between rows
   int32_t dt;     // rf_dtype
   int32_t vec;    // rows start on 16-byte boundaries
+  int64_t size;   // elements from p to the last row's end
 };
 struct RowOut {
   void* p;
@@ -53,51 +54,18 @@ struct Saved8 {
 inline bool rows_vectorised(const void* p, int64_t ld, int dt) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * int64_t(dtype_size(dt))) % 16 == 0;
 }
-inline RowView row_view(const void* p, int64_t ld, int dt) { return RowView{p, ld, dt, rows_vectorised(p, ld, dt)}; }
+inline RowView row_view(const void* p, int64_t ld, int dt, int64_t rows, int64_t features) {
+  return RowView{p, ld, dt, rows_vectorised(p, ld, dt), rows > 0 ? (rows - 1) * ld + features : 0};
+}
 inline RowOut row_out(void* p, int64_t ld, int dt) { return RowOut{p, ld, dt, rows_vectorised(p, ld, dt)}; }
 inline Saved8 saved8(const rf_saved_activation& s) {
   return Saved8{s.codes, s.scales, s.ld, s.scale_rows, s.format};
-}
-__device__ __forceinline__ RowView row_view_dev(const void* p, int64_t ld, int dt) {
-  return RowView{p, ld, dt, (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * (dt == RF_F32 ? 4 : 2)) % 16 == 0};
 }
 __device__ __forceinline__ RowOut row_out_dev(void* p, int64_t ld, int dt) {
   return RowOut{p, ld, dt, (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * (dt == RF_F32 ? 4 : 2)) % 16 == 0};
 }
 // Checks of a caller's saved activation; `what` names it in the message.
 rf_status check_saved(const rf_saved_activation* s, const char* what);
-
-// -- 8 consecutive elements of a row ----------------------------------------
-// Elements at or behind `n` read as 0 and are not written.
-__device__ __forceinline__ void load8(const RowView& t, int64_t row, int64_t col, int64_t n, float (&f)[8]) {
-  if (t.vec && col + 8 <= n) {
-    if (t.dt == RF_F32) {
-      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(t.p) + row * t.ld + col);
-      const float4 a = __ldg(p), b = __ldg(p + 1);
-      f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-    } else {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(t.p) + row * t.ld + col));
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-      if (t.dt == RF_BF16) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          f[2 * k] = __uint_as_float(w[k] << 16);
-          f[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-          f[2 * k] = x.x;
-          f[2 * k + 1] = x.y;
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = col + k < n ? ld_as_float(t.p, t.dt, row * t.ld + col + k) : 0.f;
-  }
-}
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -106,27 +74,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ void store8(const RowOut& t, int64_t row, int64_t col, int64_t n, const float (&f)[8]) {
-  if (t.vec && col + 8 <= n) {
-    if (t.dt == RF_F32) {
-      float4* p = reinterpret_cast<float4*>(static_cast<float*>(t.p) + row * t.ld + col);
-      p[0] = make_float4(f[0], f[1], f[2], f[3]);
-      p[1] = make_float4(f[4], f[5], f[6], f[7]);
-    } else {
-      uint4 u;
-      if (t.dt == RF_BF16)
-        u = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
-      else
-        u = make_uint4(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]), pack_f16(f[4], f[5]), pack_f16(f[6], f[7]));
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(t.p) + row * t.ld + col) = u;
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (col + k < n) st_from_float(t.p, t.dt, row * t.ld + col + k, f[k]);
-  }
 }
 
 // -- typed rows on 16-byte boundaries ------------------------------------------
@@ -193,6 +140,220 @@ __device__ __forceinline__ void store_vec(void* p, int64_t i, const float (&f)[8
   } else {
     *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) =
         make_uint4(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]), pack_f16(f[4], f[5]), pack_f16(f[6], f[7]));
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ Raw8<DT> pack(const float (&f)[8]) {
+  Raw8<DT> r;
+  if (DT == RF_F32) {
+    r.u[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    r.u[DT == RF_F32 ? 1 : 0] =
+        make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
+  } else if (DT == RF_BF16) {
+    r.u[0] = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+  } else {
+    r.u[0] = make_uint4(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]), pack_f16(f[4], f[5]), pack_f16(f[6], f[7]));
+  }
+  return r;
+}
+
+// -- typed rows that start and end anywhere --------------------------------------
+// One by one, 8 elements are 8 accesses that each touch every line of a warp's
+// span: 16384 x 4097 bfloat16 loaded in 187 us (now 92), 1527 x 1001 float32
+// LayerNorm forward 32 us (now 25), backward 40 (now 33).
+// So whole 16-byte pieces on their boundaries move, and registers shift them
+// into place.  A load may take in neighbouring elements of the array, never any
+// outside it: at its two ends, elements go one by one.  Stores write a row's
+// own elements only, the pieces that hang over its ends one by one.
+//
+// `i`: the first element's index behind p; `left`: how many of the row's
+// elements start there (0 or less: none).
+template <int DT>
+struct Span8 {
+  uint4 c[DT == RF_F32 ? 3 : 2];
+};
+// Elements between a 16-byte boundary and element i.
+template <int DT>
+__device__ __forceinline__ int lead(const void* p, int64_t i) {
+  constexpr int es = DT == RF_F32 ? 4 : 2;
+  return int(uint32_t(reinterpret_cast<uintptr_t>(p) / es + uint64_t(i)) & uint32_t(16 / es - 1));
+}
+// Whether the pieces that hold n elements lie within the array.
+template <int DT>
+__device__ __forceinline__ bool span_inside(int a, int64_t i, int n, int64_t size) {
+  constexpr int per = DT == RF_F32 ? 4 : 8;
+  return i >= a && i - a + (a + n + per - 1) / per * per <= size;
+}
+template <int DT>
+__device__ __forceinline__ Span8<DT> fetch_span(const RowView& t, int64_t i, int64_t left) {
+  constexpr int es = DT == RF_F32 ? 4 : 2, per = 16 / es, C = DT == RF_F32 ? 3 : 2;
+  const int a = lead<DT>(t.p, i), n = int(min(left, int64_t(8)));
+  const bool inside = span_inside<DT>(a, i, n, t.size);
+  const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(t.p) + (i - a) * es);
+  Span8<DT> s;
+#pragma unroll
+  for (int k = 0; k < C; ++k) s.c[k] = inside && n > 0 && k * per < a + n ? __ldg(q + k) : make_uint4(0, 0, 0, 0);
+  return s;
+}
+// The vector out of its pieces; zeros behind the row.
+template <int DT>
+__device__ __forceinline__ Raw8<DT> align_span(const Span8<DT>& s, const RowView& t, int64_t i, int64_t left) {
+  const int a = lead<DT>(t.p, i);
+  Raw8<DT> r;
+  if (DT == RF_F32) {
+    const uint4 z = s.c[DT == RF_F32 ? 2 : 0];
+    uint32_t w[11] = {s.c[0].x, s.c[0].y, s.c[0].z, s.c[0].w, s.c[1].x, s.c[1].y, s.c[1].z, s.c[1].w, z.x, z.y, z.z};
+#pragma unroll
+    for (int k = 0; k < 9; ++k) w[k] = a & 2 ? w[k + 2] : w[k];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = a & 1 ? w[k + 1] : w[k];
+    r.u[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    r.u[DT == RF_F32 ? 1 : 0] = make_uint4(w[4], w[5], w[6], w[7]);
+  } else {
+    uint32_t w[8] = {s.c[0].x, s.c[0].y, s.c[0].z, s.c[0].w, s.c[1].x, s.c[1].y, s.c[1].z, s.c[1].w};
+#pragma unroll
+    for (int k = 0; k < 6; ++k) w[k] = a & 4 ? w[k + 2] : w[k];
+#pragma unroll
+    for (int k = 0; k < 5; ++k) w[k] = a & 2 ? w[k + 1] : w[k];
+    const uint32_t halves = a & 1 ? 0x5432u : 0x3210u;
+    r.u[0] = make_uint4(__byte_perm(w[0], w[1], halves), __byte_perm(w[1], w[2], halves),
+                        __byte_perm(w[2], w[3], halves), __byte_perm(w[3], w[4], halves));
+  }
+  const int n = int(min(left, int64_t(8)));
+  if (n > 0 && !span_inside<DT>(a, i, n, t.size)) {
+    uint32_t w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      w[k] = 0u;
+      if (k < n) {
+        if (DT == RF_F32) w[k] = __ldg(static_cast<const uint32_t*>(t.p) + i + k);
+        else w[k] = __ldg(static_cast<const uint16_t*>(t.p) + i + k);
+      }
+    }
+    if (DT == RF_F32) {
+      r.u[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      r.u[DT == RF_F32 ? 1 : 0] = make_uint4(w[4], w[5], w[6], w[7]);
+    } else {
+      r.u[0] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+    }
+  } else if (n < 8) {
+    uint4& u = r.u[0];
+    if (DT == RF_F32) {
+      uint4& v = r.u[DT == RF_F32 ? 1 : 0];
+      u.x = n > 0 ? u.x : 0u, u.y = n > 1 ? u.y : 0u, u.z = n > 2 ? u.z : 0u, u.w = n > 3 ? u.w : 0u;
+      v.x = n > 4 ? v.x : 0u, v.y = n > 5 ? v.y : 0u, v.z = n > 6 ? v.z : 0u, v.w = 0u;
+    } else {
+      auto keep = [&](uint32_t x, int k) { return n >= k + 2 ? x : n == k + 1 ? x & 0xFFFFu : 0u; };
+      u = make_uint4(keep(u.x, 0), keep(u.y, 2), keep(u.z, 4), keep(u.w, 6));
+    }
+  }
+  return r;
+}
+// Writes a vector.  Called by all lanes of a warp; `width` neighbouring lanes
+// hold consecutive vectors of one row, and each writes the pieces that end
+// within its own, with the first elements from the lane before.
+template <int DT>
+__device__ __forceinline__ void store_span(void* p, int64_t i, int64_t left, const Raw8<DT>& r, int width = 32) {
+  constexpr int es = DT == RF_F32 ? 4 : 2;
+  const int a = lead<DT>(p, i), lane = int(threadIdx.x + blockDim.x * threadIdx.y) & (width - 1);
+  uint8_t* q = static_cast<uint8_t*>(p) + (i - a) * es;
+  bool head, next;  // the piece that starts at q, and the one that holds this vector's last elements
+  if (DT == RF_F32) {
+    const uint4 u = r.u[DT == RF_F32 ? 1 : 0];
+    uint32_t w[11] = {0, 0, 0, r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w, u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int k = 0; k < 3; ++k) w[k] = __shfl_up_sync(0xFFFFFFFFu, w[k + 8], 1);
+#pragma unroll
+    for (int k = 10; k >= 2; --k) w[k] = a & 2 ? w[k - 2] : w[k];
+#pragma unroll
+    for (int k = 10; k >= 3; --k) w[k] = a & 1 ? w[k - 1] : w[k];
+    head = left >= 4 - a && (a == 0 || lane != 0);
+    const bool mid = left >= 8 - a;
+    next = a == 0 || (lane != width - 1 && left - 8 >= 4 - a);
+    if (head) *reinterpret_cast<uint4*>(q) = make_uint4(w[3], w[4], w[5], w[6]);
+    if (mid) *reinterpret_cast<uint4*>(q + 16) = make_uint4(w[7], w[8], w[9], w[10]);
+    if (head && mid && next) return;
+    const uint32_t f[8] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w, u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < left && !(k < 4 - a ? head : k < 8 - a ? mid : next)) static_cast<uint32_t*>(p)[i + k] = f[k];
+  } else {
+    const uint32_t f[4] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w};
+    uint32_t w[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] = __shfl_up_sync(0xFFFFFFFFu, f[k], 1);
+      w[4 + k] = f[k];
+    }
+#pragma unroll
+    for (int k = 7; k >= 2; --k) w[k] = a & 4 ? w[k - 2] : w[k];
+#pragma unroll
+    for (int k = 7; k >= 3; --k) w[k] = a & 2 ? w[k - 1] : w[k];
+    const uint32_t halves = a & 1 ? 0x5432u : 0x7654u;
+    head = left >= 8 - a && (a == 0 || lane != 0);
+    next = a == 0 || (lane != width - 1 && left - 8 >= 8 - a);
+    if (head)
+      *reinterpret_cast<uint4*>(q) = make_uint4(__byte_perm(w[3], w[4], halves), __byte_perm(w[4], w[5], halves),
+                                                __byte_perm(w[5], w[6], halves), __byte_perm(w[6], w[7], halves));
+    if (head && next) return;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < left && !(k < 8 - a ? head : next))
+        static_cast<uint16_t*>(p)[i + k] = uint16_t(f[k >> 1] >> (16 * (k & 1)));
+  }
+}
+
+// -- the same with the type known at run time -------------------------------------
+// 8 elements of a row; those at or behind `n` read as 0.
+template <int DT>
+__device__ __forceinline__ void load8_as(const RowView& t, int64_t i, int64_t col, int64_t n, float (&f)[8]) {
+  if (t.vec && col + 8 <= n) unpack<DT>(load_raw<DT>(t.p, i), f);
+  else unpack<DT>(align_span<DT>(fetch_span<DT>(t, i, n - col), t, i, n - col), f);
+}
+__device__ __forceinline__ void load8(const RowView& t, int64_t row, int64_t col, int64_t n, float (&f)[8]) {
+  const int64_t i = row * t.ld + col;
+  if (t.dt == RF_F32) load8_as<RF_F32>(t, i, col, n, f);
+  else if (t.dt == RF_BF16) load8_as<RF_BF16>(t, i, col, n, f);
+  else load8_as<RF_F16>(t, i, col, n, f);
+}
+// 8 values of a parameter or a gate with d elements: short code and few
+// registers, for they are read beside a row, from near caches.
+__device__ __forceinline__ void load8_param(const void* p, int dt, int64_t col, int64_t d, float (&f)[8]) {
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && col + 8 <= d) {
+    if (dt == RF_F32) unpack<RF_F32>(load_raw<RF_F32>(p, col), f);
+    else if (dt == RF_BF16) unpack<RF_BF16>(load_raw<RF_BF16>(p, col), f);
+    else unpack<RF_F16>(load_raw<RF_F16>(p, col), f);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = col + k < d ? ld_as_float(p, dt, col + k) : 0.f;
+  }
+}
+// Writes 8 elements but those at or behind `n`; one lane alone.
+__device__ __forceinline__ void store8(const RowOut& t, int64_t row, int64_t col, int64_t n, const float (&f)[8]) {
+  const int64_t i = row * t.ld + col;
+  if (t.vec && col + 8 <= n) {
+    if (t.dt == RF_F32) store_vec<RF_F32>(t.p, i, f);
+    else if (t.dt == RF_BF16) store_vec<RF_BF16>(t.p, i, f);
+    else store_vec<RF_F16>(t.p, i, f);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (col + k < n) st_from_float(t.p, t.dt, i + k, f[k]);
+  }
+}
+// The same by a whole warp whose lanes hold consecutive vectors.
+__device__ __forceinline__ void store8_warp(const RowOut& t, int64_t row, int64_t col, int64_t n,
+                                            const float (&f)[8]) {
+  const int64_t i = row * t.ld + col;
+  if (t.vec && n % 8 == 0) {
+    if (col < n) store8(t, row, col, n, f);
+  } else if (t.dt == RF_F32) {
+    store_span<RF_F32>(t.p, i, n - col, pack<RF_F32>(f));
+  } else if (t.dt == RF_BF16) {
+    store_span<RF_BF16>(t.p, i, n - col, pack<RF_BF16>(f));
+  } else {
+    store_span<RF_F16>(t.p, i, n - col, pack<RF_F16>(f));
   }
 }
 

@@ -4,7 +4,7 @@
 //   x' = x + s a(gamma) N_post(b),   y = N_pre(x')
 //
 // The C entry points and the kernels for every type and width; the usual
-// types up to 8192 features go through rf_block_norm_typed.cu's kernels, which
+// types up to 8192 features go through rf_block_norm_typed.cuh's kernels, which
 // hold their rows the same way and are 2 to 3 times as fast.
 //
 // Both directions are bound by HBM: a row is read once, held in registers
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : 512) k_norm_fwd(co
       scale8(c, col, s);
 #pragma unroll
       for (int k = 0; k < 8; ++k) x[v][k] = fmaf(b[v][k] * w[k], s[k], x[v][k]);
-      if (A.x_out.p) store8(A.x_out, row, col, c.d, x[v]);
+      if (A.x_out.p) store8_warp(A.x_out, row, col, c.d, x[v]);
       if (A.sx.codes) {
         float t[8];
 #pragma unroll
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : 512) k_norm_fwd(co
 #pragma unroll
       for (int k = 0; k < 8; ++k) x[v][k] += w[k];
     }
-    store8(A.y, row, col, c.d, x[v]);
+    store8_warp(A.y, row, col, c.d, x[v]);
     if (A.sy.codes) {
       round8(A.y.dt, x[v]);
       save_row8(A.sy, row, col, c.d, x[v]);
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : 512) k_norm_bwd(co
           for (int k = 0; k < 8; ++k) e[v][k] = fmaf(r, g[v][k] - mg - x[v][k] * mgn, e[v][k]);
       }
 #pragma unroll
-      for (int v = 0; v < V; ++v) store8(A.dx, row, int64_t(v * team + lane) * 8, c.d, e[v]);
+      for (int v = 0; v < V; ++v) store8_warp(A.dx, row, int64_t(v * team + lane) * 8, c.d, e[v]);
       if (!has_b) continue;
 
 #pragma unroll
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : 512) k_norm_bwd(co
           for (int k = 0; k < 8; ++k) e[v][k] = rb * (e[v][k] - mh - x[v][k] * mhm);
       }
 #pragma unroll
-      for (int v = 0; v < V; ++v) store8(A.db, row, int64_t(v * team + lane) * 8, c.d, e[v]);
+      for (int v = 0; v < V; ++v) store8_warp(A.db, row, int64_t(v * team + lane) * 8, c.d, e[v]);
     }
 
     if (!A.partial) continue;
@@ -585,7 +585,9 @@ Common common_of(const rf_block_norm& p) {
   c.gate_act = p.gate_act;
   return c;
 }
-RowView view(const rf_rows* t) { return present(t) && t->data ? row_view(t->data, t->ld, t->dtype) : RowView{}; }
+RowView view(const rf_rows* t, const rf_block_norm& p) {
+  return present(t) && t->data ? row_view(t->data, t->ld, t->dtype, p.rows, p.features) : RowView{};
+}
 RowOut out(const rf_rows* t) {
   return present(t) ? row_out(const_cast<void*>(t->data), t->ld, t->dtype) : RowOut{};
 }
@@ -660,9 +662,9 @@ extern "C" rf_status rf_block_norm_forward(const rf_block_norm* p, const rf_rows
   if (!has_b && !has_y && !saved_x) return RF_OK;
   FwdArgs A{};
   A.c = common_of(*p);
-  A.x = view(x);
+  A.x = view(x, *p);
   if (has_b) {
-    A.b = view(branch);
+    A.b = view(branch, *p);
     A.x_out = out(x_out);
   }
   if (has_y) A.y = out(y);
@@ -716,15 +718,15 @@ extern "C" rf_status rf_block_norm_backward(const rf_block_norm* p, const rf_row
   if (rows > 0) {
     BwdArgs A{};
     A.c = common_of(*p);
-    if (has_gx) A.gx = view(grad_x);
+    if (has_gx) A.gx = view(grad_x, *p);
     if (has_gy) {
-      A.gy = view(grad_y);
+      A.gy = view(grad_y, *p);
       if (x->saved) A.sx = saved8(*x->saved);
-      else A.x = view(x);
+      else A.x = view(x, *p);
     }
     if (has_b) {
       if (branch->saved) A.sb = saved8(*branch->saved);
-      else A.b = view(branch);
+      else A.b = view(branch, *p);
       A.db = out(out_branch);
     }
     A.dx = out(out_x);

@@ -52,8 +52,7 @@ __device__ __forceinline__ void param8(const Param& w, int64_t col, int64_t d, f
     for (int k = 0; k < 8; ++k) f[k] = absent;
     return;
   }
-  const RowView v{w.p, 0, w.dt, (reinterpret_cast<uintptr_t>(w.p) & 15) == 0};
-  load8(v, 0, col, d, f);
+  load8_param(w.p, w.dt, col, d, f);
 }
 __device__ __forceinline__ float gate_value(float g, int act) {
   return act == RF_GATE_SIGMOID ? 1.f / (1.f + expf(-g)) : act == RF_GATE_TANH ? tanhf(g) : g;
@@ -71,7 +70,8 @@ __device__ __forceinline__ void gate8(const Common& c, int64_t row, int64_t col,
   }
   const int64_t g = row / c.gate_rows;
   if (c.gate_per_channel) {
-    load8(row_view_dev(c.gate.p, c.d, c.gate.dt), g, col, c.d, f);
+    const int es = c.gate.dt == RF_F32 ? 4 : 2;
+    load8_param(static_cast<const uint8_t*>(c.gate.p) + g * c.d * es, c.gate.dt, col, c.d, f);
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[k] = gate_value(f[k], c.gate_act);
   } else {
@@ -90,7 +90,7 @@ __device__ __forceinline__ void scale8(const Common& c, int64_t col, float (&f)[
   for (int k = 0; k < 8; ++k) f[k] = s;
 }
 
-// The typed kernels (rf_block_norm_typed.cu): arrays of one of four pairs of
+// The typed kernels (rf_block_norm_typed.cuh): arrays of one of four pairs of
 // element types.  Each returns true when it took the call.
 struct TypedTeam {
   int threads, vectors, teams;  // threads of a row's team, 8-feature vectors per thread, teams per CTA

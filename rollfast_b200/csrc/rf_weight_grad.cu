@@ -714,7 +714,7 @@ extern "C" rf_status rf_weight_gradient(const rf_saved_activation* saved, const 
       const int tx = int(nv < 256 ? nv : 256), ty = 256 / tx;
       const int64_t gx = std::min<int64_t>(ceil_div(rows, ty), 65535);
       k_grad_terms<<<dim3(unsigned(gx), unsigned(ceil_div(nv, tx))), dim3(unsigned(tx), unsigned(ty)), 0, st>>>(
-          row_view(grad_out, ld_grad, grad_dtype), reinterpret_cast<uint16_t*>(ws + p.x_bytes), rows, n_out,
+          row_view(grad_out, ld_grad, grad_dtype, rows, n_out), reinterpret_cast<uint16_t*>(ws + p.x_bytes), rows, n_out,
           p.ld_terms, p.terms);
       RF_TRY(check_launch("k_grad_terms"));
       g = ws + p.x_bytes;
