@@ -161,7 +161,7 @@ __device__ __forceinline__ Raw8<DT> pack(const float (&f)[8]) {
 // -- typed rows that start and end anywhere --------------------------------------
 // One by one, 8 elements are 8 accesses that each touch every line of a warp's
 // span: 16384 x 4097 bfloat16 loaded in 187 us (now 92), 1527 x 1001 float32
-// LayerNorm forward 32 us (now 25), backward 40 (now 33).
+// LayerNorm backward 40 us (now 33).
 // So whole 16-byte pieces on their boundaries move, and registers shift them
 // into place.  A load may take in neighbouring elements of the array, never any
 // outside it: at its two ends, elements go one by one.  Stores write a row's

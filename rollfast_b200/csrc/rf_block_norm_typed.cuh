@@ -5,16 +5,17 @@
 //
 // Bound by HBM.  A row belongs to a team of whole warps, 8 V features to a
 // thread, and a CTA holds several teams when rows are short.  CTAs stay and
-// walk down the rows with the next row's loads in flight, and a thread keeps
-// the parameters of its columns in registers, scale, gate and weight folded
-// into one factor.  Rows that start off 16-byte boundaries, or are no whole
-// number of vectors wide, are shifted into place (rf_act8.cuh).
+// walk down the rows, where registers allow with the next row's loads in
+// flight; scale, gate and weight of a column are folded into one factor.  Rows
+// that start off 16-byte boundaries, or are no whole number of vectors wide,
+// are shifted into place (rf_act8.cuh).
 //
-// Measured on a B200 (a copy: 6549 GB/s), 16384 x 4096 bfloat16 RMS: forward 100 us (5.4 TB/s), with
-// the 8-bit copies 172; backward 170 us (4.7 TB/s), from saved activations 186.
-// With copies and backward, the issue slots are the bound, not HBM.  Backward
-// beyond 4096 features a thread holds two vectors, which do not fit its 128
-// registers (700 to 1400 bytes spilled): 8192 x 5120 in 194 us, 2.1 TB/s.
+// Measured on a B200 (a copy: 6549 GB/s), 16384 x 4096 bfloat16 RMS: forward
+// 98 us (5.5 TB/s), with the 8-bit copies 174; backward 168 us (4.8 TB/s), from
+// saved activations 185.  With copies and backward, the issue slots are the
+// bound, not HBM.  Backward beyond 4096 features a thread holds two vectors,
+// which do not fit its 128 registers (700 to 1400 bytes spilled): 8192 x 5120
+// in 194 us, 2.1 TB/s.
 #pragma once
 
 #include <type_traits>
@@ -27,7 +28,8 @@ namespace bn {
 namespace {
 
 constexpr int kTypedThreads = 512;
-constexpr int kMaxTeams = 8;
+constexpr int kFwdThreads = 768;  // forward, where registers suffice for more warps
+constexpr int kMaxTeams = 12;
 constexpr int64_t kMaxTyped = 2 * kTypedThreads * 8;
 constexpr int kFwdVectors = 2;  // vectors per thread, forward
 
@@ -239,10 +241,10 @@ bool with_types(int xt, int bt, bool vec, F&& f) {
   return true;
 }
 
-TypedTeam team_for(int64_t d, int vectors) {
+TypedTeam team_for(int64_t d, int vectors, int threads = kTypedThreads) {
   const int64_t nv = ceil_div(d, kPanel8) * (kPanel8 / 8);  // whole panels, for a saved row's last one
   const int t = int(std::min<int64_t>(round_up(ceil_div(nv, vectors), 32), kTypedThreads));
-  return {t, vectors, std::min(kTypedThreads / t, kMaxTeams)};
+  return {t, vectors, std::min(threads / t, kMaxTeams)};
 }
 
 }  // namespace
