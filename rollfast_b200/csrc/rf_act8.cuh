@@ -304,32 +304,26 @@ __device__ __forceinline__ void store_span(void* p, int64_t i, int64_t left, con
   }
 }
 
-// -- the same with the type known at run time -------------------------------------
-// 8 elements of a row; those at or behind `n` read as 0.
-template <int DT>
-__device__ __forceinline__ void load8_as(const RowView& t, int64_t i, int64_t col, int64_t n, float (&f)[8]) {
-  if (t.vec && col + 8 <= n) unpack<DT>(load_raw<DT>(t.p, i), f);
-  else unpack<DT>(align_span<DT>(fetch_span<DT>(t, i, n - col), t, i, n - col), f);
-}
+// -- 8 elements with the type known at run time -----------------------------------
+// Short code, for kernels of any combination of types and for parameters:
+// shifted pieces of three types took no less time there.  Those at or behind
+// `n` read as 0.
 __device__ __forceinline__ void load8(const RowView& t, int64_t row, int64_t col, int64_t n, float (&f)[8]) {
   const int64_t i = row * t.ld + col;
-  if (t.dt == RF_F32) load8_as<RF_F32>(t, i, col, n, f);
-  else if (t.dt == RF_BF16) load8_as<RF_BF16>(t, i, col, n, f);
-  else load8_as<RF_F16>(t, i, col, n, f);
-}
-// 8 values of a parameter or a gate with d elements: short code and few
-// registers, for they are read beside a row, from near caches.
-__device__ __forceinline__ void load8_param(const void* p, int dt, int64_t col, int64_t d, float (&f)[8]) {
-  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && col + 8 <= d) {
-    if (dt == RF_F32) unpack<RF_F32>(load_raw<RF_F32>(p, col), f);
-    else if (dt == RF_BF16) unpack<RF_BF16>(load_raw<RF_BF16>(p, col), f);
-    else unpack<RF_F16>(load_raw<RF_F16>(p, col), f);
+  if (t.vec && col + 8 <= n) {
+    if (t.dt == RF_F32) unpack<RF_F32>(load_raw<RF_F32>(t.p, i), f);
+    else if (t.dt == RF_BF16) unpack<RF_BF16>(load_raw<RF_BF16>(t.p, i), f);
+    else unpack<RF_F16>(load_raw<RF_F16>(t.p, i), f);
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = col + k < d ? ld_as_float(p, dt, col + k) : 0.f;
+    for (int k = 0; k < 8; ++k) f[k] = col + k < n ? ld_as_float(t.p, t.dt, i + k) : 0.f;
   }
 }
-// Writes 8 elements but those at or behind `n`; one lane alone.
+// 8 values of a parameter or a gate with d elements.
+__device__ __forceinline__ void load8_param(const void* p, int dt, int64_t col, int64_t d, float (&f)[8]) {
+  load8(RowView{p, 0, dt, (reinterpret_cast<uintptr_t>(p) & 15) == 0, d}, 0, col, d, f);
+}
+// Writes 8 elements but those at or behind `n`.
 __device__ __forceinline__ void store8(const RowOut& t, int64_t row, int64_t col, int64_t n, const float (&f)[8]) {
   const int64_t i = row * t.ld + col;
   if (t.vec && col + 8 <= n) {
@@ -342,21 +336,6 @@ __device__ __forceinline__ void store8(const RowOut& t, int64_t row, int64_t col
       if (col + k < n) st_from_float(t.p, t.dt, i + k, f[k]);
   }
 }
-// The same by a whole warp whose lanes hold consecutive vectors.
-__device__ __forceinline__ void store8_warp(const RowOut& t, int64_t row, int64_t col, int64_t n,
-                                            const float (&f)[8]) {
-  const int64_t i = row * t.ld + col;
-  if (t.vec && n % 8 == 0) {
-    if (col < n) store8(t, row, col, n, f);
-  } else if (t.dt == RF_F32) {
-    store_span<RF_F32>(t.p, i, n - col, pack<RF_F32>(f));
-  } else if (t.dt == RF_BF16) {
-    store_span<RF_BF16>(t.p, i, n - col, pack<RF_BF16>(f));
-  } else {
-    store_span<RF_F16>(t.p, i, n - col, pack<RF_F16>(f));
-  }
-}
-
 // -- pairs ------------------------------------------------------------------
 // sm_100 multiplies and adds two float32 in one instruction; these kernels are
 // short of issue slots, not of arithmetic.  Same roundings as one by one.

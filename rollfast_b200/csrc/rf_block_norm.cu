@@ -5,7 +5,9 @@
 //
 // The C entry points and the kernels for every type and width; the usual
 // types up to 8192 features go through rf_block_norm_typed.cuh's kernels, which
-// hold their rows the same way and are 2 to 3 times as fast.
+// hold their rows the same way and are several times as fast (these: 8192 x
+// 12288 bfloat16 RMS forward 939 us, 0.86 TB/s, bound by the parameters' reads
+// and conversions in every row).
 //
 // Both directions are bound by HBM: a row is read once, held in registers
 // while its statistics are formed, and each output is written once.  A row
@@ -130,7 +132,7 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : 512) k_norm_fwd(co
       scale8(c, col, s);
 #pragma unroll
       for (int k = 0; k < 8; ++k) x[v][k] = fmaf(b[v][k] * w[k], s[k], x[v][k]);
-      if (A.x_out.p) store8_warp(A.x_out, row, col, c.d, x[v]);
+      if (A.x_out.p) store8(A.x_out, row, col, c.d, x[v]);
       if (A.sx.codes) {
         float t[8];
 #pragma unroll
@@ -159,7 +161,7 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : 512) k_norm_fwd(co
 #pragma unroll
       for (int k = 0; k < 8; ++k) x[v][k] += w[k];
     }
-    store8_warp(A.y, row, col, c.d, x[v]);
+    store8(A.y, row, col, c.d, x[v]);
     if (A.sy.codes) {
       round8(A.y.dt, x[v]);
       save_row8(A.sy, row, col, c.d, x[v]);
@@ -233,7 +235,7 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : 512) k_norm_bwd(co
           for (int k = 0; k < 8; ++k) e[v][k] = fmaf(r, g[v][k] - mg - x[v][k] * mgn, e[v][k]);
       }
 #pragma unroll
-      for (int v = 0; v < V; ++v) store8_warp(A.dx, row, int64_t(v * team + lane) * 8, c.d, e[v]);
+      for (int v = 0; v < V; ++v) store8(A.dx, row, int64_t(v * team + lane) * 8, c.d, e[v]);
       if (!has_b) continue;
 
 #pragma unroll
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(kWarp ? 32 * kWarpsPerCta : 512) k_norm_bwd(co
           for (int k = 0; k < 8; ++k) e[v][k] = rb * (e[v][k] - mh - x[v][k] * mhm);
       }
 #pragma unroll
-      for (int v = 0; v < V; ++v) store8_warp(A.db, row, int64_t(v * team + lane) * 8, c.d, e[v]);
+      for (int v = 0; v < V; ++v) store8(A.db, row, int64_t(v * team + lane) * 8, c.d, e[v]);
     }
 
     if (!A.partial) continue;

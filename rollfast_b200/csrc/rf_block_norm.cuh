@@ -98,6 +98,7 @@ struct TypedTeam {
 TypedTeam typed_team(int64_t d);
 bool try_typed_fwd(const rf_block_norm& p, const FwdArgs& A, cudaStream_t st);
 bool try_typed_bwd(const rf_block_norm& p, const BwdArgs& A, bool bias, cudaStream_t st);
+bool try_typed_layer_bwd(const rf_block_norm& p, const BwdArgs& A, bool bias, cudaStream_t st);  // LayerNorm only
 
 }  // namespace bn
 }  // namespace rf
