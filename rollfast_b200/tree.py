@@ -35,47 +35,51 @@ class _Node:
 _LEAF = _Node("leaf", None, ())
 
 
-def tree_flatten(tree: Any, is_leaf: Callable[[Any], bool] | None = None):
-    leaves: list = []
+# The recursions are module functions: a nested function that names itself is a
+# reference cycle, which kept a whole tree of arrays (an update tree of 30 GiB)
+# allocated after its last use, until the garbage collector happened to run.
 
-    def rec(x):
-        if is_leaf is not None and is_leaf(x):
-            leaves.append(x)
-            return _LEAF
-        if x is None:
-            return _Node("none", None, ())
-        if isinstance(x, MaskedNode):
-            return _Node("masked", None, ())
-        if isinstance(x, dict):
-            keys = list(x.keys())
-            return _Node("dict", keys, [rec(x[k]) for k in keys])
-        if _is_namedtuple(x):
-            return _Node("namedtuple", type(x), [rec(v) for v in x])
-        if isinstance(x, (list, tuple)):
-            return _Node(type(x), None, [rec(v) for v in x])
+
+def _flatten(x: Any, is_leaf, leaves: list) -> _Node:
+    if is_leaf is not None and is_leaf(x):
         leaves.append(x)
         return _LEAF
+    if x is None:
+        return _Node("none", None, ())
+    if isinstance(x, MaskedNode):
+        return _Node("masked", None, ())
+    if isinstance(x, dict):
+        keys = list(x.keys())
+        return _Node("dict", keys, [_flatten(x[k], is_leaf, leaves) for k in keys])
+    if _is_namedtuple(x):
+        return _Node("namedtuple", type(x), [_flatten(v, is_leaf, leaves) for v in x])
+    if isinstance(x, (list, tuple)):
+        return _Node(type(x), None, [_flatten(v, is_leaf, leaves) for v in x])
+    leaves.append(x)
+    return _LEAF
 
-    return leaves, rec(tree)
+
+def tree_flatten(tree: Any, is_leaf: Callable[[Any], bool] | None = None):
+    leaves: list = []
+    return leaves, _flatten(tree, is_leaf, leaves)
+
+
+def _unflatten(n: _Node, it) -> Any:
+    if n is _LEAF or n.kind == "leaf":
+        return next(it)
+    if n.kind == "none":
+        return None
+    if n.kind == "masked":
+        return MaskedNode()
+    if n.kind == "dict":
+        return {k: _unflatten(c, it) for k, c in zip(n.meta, n.children)}
+    if n.kind == "namedtuple":
+        return n.meta(*[_unflatten(c, it) for c in n.children])
+    return n.kind(_unflatten(c, it) for c in n.children)
 
 
 def tree_unflatten(treedef: _Node, leaves) -> Any:
-    it = iter(leaves)
-
-    def rec(n: _Node):
-        if n is _LEAF or n.kind == "leaf":
-            return next(it)
-        if n.kind == "none":
-            return None
-        if n.kind == "masked":
-            return MaskedNode()
-        if n.kind == "dict":
-            return {k: rec(c) for k, c in zip(n.meta, n.children)}
-        if n.kind == "namedtuple":
-            return n.meta(*[rec(c) for c in n.children])
-        return n.kind(rec(c) for c in n.children)
-
-    return rec(treedef)
+    return _unflatten(treedef, iter(leaves))
 
 
 def tree_leaves(tree: Any, is_leaf=None) -> list:
@@ -90,27 +94,27 @@ def tree_map(fn: Callable, tree: Any, *rest: Any, is_leaf=None) -> Any:
     return tree_unflatten(treedef, [fn(*xs) for xs in zip(leaves, *others)])
 
 
+def _collect(n: _Node, x: Any, out: list) -> None:
+    if n is _LEAF or n.kind == "leaf":
+        out.append(x)
+        return
+    if n.kind in ("none", "masked"):
+        return
+    if n.kind == "dict":
+        if not isinstance(x, dict) or set(x.keys()) != set(n.meta):
+            raise ValueError("tree structures do not match")
+        for k, c in zip(n.meta, n.children):
+            _collect(c, x[k], out)
+        return
+    if not isinstance(x, (list, tuple)) or len(x) != len(n.children):
+        raise ValueError("tree structures do not match")
+    for c, v in zip(n.children, x):
+        _collect(c, v, out)
+
+
 def _flatten_up_to(treedef: _Node, tree: Any) -> list:
     out: list = []
-
-    def rec(n: _Node, x):
-        if n is _LEAF or n.kind == "leaf":
-            out.append(x)
-            return
-        if n.kind in ("none", "masked"):
-            return
-        if n.kind == "dict":
-            if not isinstance(x, dict) or set(x.keys()) != set(n.meta):
-                raise ValueError("tree structures do not match")
-            for k, c in zip(n.meta, n.children):
-                rec(c, x[k])
-            return
-        if not isinstance(x, (list, tuple)) or len(x) != len(n.children):
-            raise ValueError("tree structures do not match")
-        for c, v in zip(n.children, x):
-            rec(c, v)
-
-    rec(treedef, tree)
+    _collect(treedef, tree, out)
     return out
 
 
