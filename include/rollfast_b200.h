@@ -411,6 +411,7 @@ typedef struct rf_rows {
 } rf_rows;
 
 /* branch.data NULL: y = N_pre(x) alone (x_out unused).  y.data NULL: x' alone.
+ * Parameters of the part that is left out must be absent.
  * saved_* (each may be NULL) receive x', b and y in 8 bits, exactly as
  * rf_save_activation of the stored arrays would. */
 rf_status rf_block_norm_forward(const rf_block_norm* p, const rf_rows* x, const rf_rows* branch, const rf_rows* x_out,

@@ -116,6 +116,20 @@ def _describe(shape, kind, eps, post_norm, params, gate_activation):
     return p, keep
 
 
+def _refuse_unused(branch, given: dict, pre_norm: bool = True) -> None:
+    """Parameters of a part that the call leaves out: without an error, a
+    forgotten branch or norm would go unnoticed."""
+    if branch is None:
+        extra = [n for n in ("post_weight", "post_bias", "gate") if given[n] is not None]
+        if isinstance(given["residual_scale"], torch.Tensor):
+            extra.append("residual_scale")
+        if extra:
+            raise ValueError(f"{', '.join(extra)} given without a branch")
+    extra = [n for n in ("pre_weight", "pre_bias") if given[n] is not None]
+    if extra and not pre_norm:
+        raise ValueError(f"{', '.join(extra)} given with pre_norm=False")
+
+
 def _rows(t, what: str, shape):
     """(RfRows, what must stay alive)"""
     if isinstance(t, SavedActivation):
@@ -151,8 +165,9 @@ def block_norm_forward(x: torch.Tensor, branch: torch.Tensor | None = None, *, k
     """``x' = x + residual_scale * act(gate) * N_post(branch)``, ``y = N_pre(x')``.
 
     Without ``branch`` (before the first block) ``y = N_pre(x)``; with
-    ``pre_norm=False`` (after the last) there is no ``y``; with
-    ``post_norm=False`` the branch is added as it is.  ``gate`` broadcasts
+    ``pre_norm=False`` (after the last) there is no ``y``; tensors of the part
+    that is left out are refused.  With ``post_norm=False`` the branch is added
+    as it is.  ``gate`` broadcasts
     against ``x``: equal to it along the first axes, 1 along the rest, d or 1
     along the last -- (d,), (batch, 1, d), (batch, tokens, 1), ``x``'s own
     shape.  ``residual_scale``: a number, (d,) or one element.  x' has ``x``'s
@@ -162,6 +177,7 @@ def block_norm_forward(x: torch.Tensor, branch: torch.Tensor | None = None, *, k
     shape = tuple(x.shape)
     given = dict(pre_weight=pre_weight, pre_bias=pre_bias, post_weight=post_weight, post_bias=post_bias, gate=gate,
                  residual_scale=residual_scale)
+    _refuse_unused(branch, given, pre_norm)
     p, keep = _describe(shape, kind, eps, post_norm, given, gate_activation)
     if save is not None:
         _format_code(save)
@@ -206,12 +222,7 @@ def block_norm_backward(grad_x: torch.Tensor | None, grad_y: torch.Tensor | None
     given = dict(pre_weight=pre_weight, pre_bias=pre_bias, post_weight=post_weight, post_bias=post_bias, gate=gate,
                  residual_scale=residual_scale)
     p, keep = _describe(shape, kind, eps, post_norm, given, gate_activation)
-    if branch is None:
-        extra = [n for n in ("post_weight", "post_bias", "gate") if given[n] is not None]
-        if isinstance(residual_scale, torch.Tensor):
-            extra.append("residual_scale")
-        if extra:
-            raise ValueError(f"{', '.join(extra)} given without a branch")
+    _refuse_unused(branch, given)
     device = x.device
     for name, t in (("grad_x", grad_x), ("grad_y", grad_y)):
         if t is not None:

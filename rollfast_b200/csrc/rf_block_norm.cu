@@ -651,9 +651,13 @@ extern "C" rf_status rf_block_norm_forward(const rf_block_norm* p, const rf_rows
     RF_TRY(check_array(x_out, rows, d, "rf_block_norm_forward: x_out", false));
   } else if (saved_branch) {
     return fail(RF_EINVAL, "rf_block_norm_forward: saved_branch without a branch");
+  } else if (p->post_weight.value || p->post_bias.value || p->gate.value || p->residual_scale.value) {
+    return fail(RF_EINVAL, "rf_block_norm_forward: the branch's parameters without a branch");
   }
   if (has_y) RF_TRY(check_array(y, rows, d, "rf_block_norm_forward: y", false));
   else if (saved_y) return fail(RF_EINVAL, "rf_block_norm_forward: saved_y without y");
+  else if (p->pre_weight.value || p->pre_bias.value)
+    return fail(RF_EINVAL, "rf_block_norm_forward: pre_weight and pre_bias without y");
   const rf_saved_activation* saved[3] = {saved_x, saved_branch, saved_y};
   for (const rf_saved_activation* s : saved) {
     if (!s) continue;
