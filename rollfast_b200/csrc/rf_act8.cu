@@ -711,7 +711,10 @@ extern "C" rf_status rf_load_activation(const rf_saved_activation* saved, void* 
   RF_TRY(check_rows(out, ldo, dtype, saved->rows, saved->features, "rf_load_activation: out"));
   if (saved->rows == 0) return RF_OK;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (typed(saved->features, out, ldo, dtype)) {
+  // Typed float32 column tiles are 1024 features, not 2048: beyond 65535 of
+  // them (grid.y) the simple kernel takes the row.
+  const bool fits = dtype != RF_F32 || saved->features <= int64_t(65535) * kThreads * 4;
+  if (fits && typed(saved->features, out, ldo, dtype)) {
     with_types(dtype, saved->format, [&](auto dt, auto fmt) {
       constexpr int DT = decltype(dt)::value;
       constexpr auto kernel = k_load_typed<DT, decltype(fmt)::value>;

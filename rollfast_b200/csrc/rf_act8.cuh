@@ -27,7 +27,7 @@ namespace rf {
 constexpr int kBlock8 = 32;       // features that share a step
 constexpr int kPanel8 = 128;      // features per panel of steps
 constexpr uint32_t kNanStep = 255u;
-constexpr int64_t kMaxFeatures = int64_t(1) << 26;  // keeps column tiles inside a grid's 65535 in y
+constexpr int64_t kMaxFeatures = int64_t(1) << 26;  // keeps column tiles of 2048 features inside a grid's 65535 in y
 
 // A device view of a row-strided array of one of the float types.
 struct RowView {
