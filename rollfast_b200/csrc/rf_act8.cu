@@ -416,9 +416,17 @@ __global__ void __launch_bounds__(kThreads) k_load(Saved8 in, RowOut out, int64_
 }
 
 // sigma(g) from one exponential that cannot overflow, so that very negative
-// g fade out through the subnormals; 1 + e lies in [1, 2], where the
-// approximate reciprocal is off by at most one unit.
+// g fade out through the subnormals; 1 + e lies in [1, 2].
+// Float32 arrays: expf and a rounded division, at most 4 units off throughout.
+// 16-bit arrays: the fast exponential, off by up to 2 + 1.2 |g| units of
+// float32, and the approximate reciprocal, off by one: at |g| = 80 that is
+// 2^-16 of the value, where bfloat16 rounds by 2^-9 and float16 by 2^-12.
+template <int DT>
 __device__ __forceinline__ float sigmoid(float g) {
+  if (DT == RF_F32) {
+    const float e = expf(-fabsf(g));
+    return (g < 0.f ? e : 1.f) / (1.f + e);
+  }
   const float e = __expf(-fabsf(g));
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
@@ -470,7 +478,7 @@ __global__ void __launch_bounds__(kThreads) k_swiglu_fwd_typed(const void* gate,
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        put_pair(g, k, __fmul2_rn(__fmul2_rn(pair(g, k), make_float2(sigmoid(g[2 * k]), sigmoid(g[2 * k + 1]))),
+        put_pair(g, k, __fmul2_rn(__fmul2_rn(pair(g, k), make_float2(sigmoid<DT>(g[2 * k]), sigmoid<DT>(g[2 * k + 1]))),
                                   pair(u, k)));
       if (data && r < n) ch.store(r, g);
     }
@@ -483,10 +491,11 @@ __global__ void __launch_bounds__(kThreads) k_swiglu_fwd_typed(const void* gate,
 
 // h = silu(g) u; dh/du = silu(g); dh/dg = u s (1 + g (1 - s)).  g and u become
 // the gradients.
+template <int DT>
 __device__ __forceinline__ void swiglu_back8(const float (&d)[8], float (&g)[8], float (&u)[8], float (&h)[8]) {
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const float2 s = make_float2(sigmoid(g[2 * k]), sigmoid(g[2 * k + 1]));
+    const float2 s = make_float2(sigmoid<DT>(g[2 * k]), sigmoid<DT>(g[2 * k + 1]));
     const float2 x = pair(u, k), y = pair(d, k);
     const float2 a = __fmul2_rn(pair(g, k), s);
     put_pair(h, k, __fmul2_rn(a, x));
@@ -554,7 +563,7 @@ __global__ void __launch_bounds__(kThreads) k_swiglu_bwd_typed(const void* dh, i
       decode4(ru[r].y, up.format, u + 4);
       mul8(g, both(fg[r]));
       mul8(u, both(fu[r]));
-      swiglu_back8(d, g, u, h);
+      swiglu_back8<DT>(d, g, u, h);
       if (kSave) {
         const uint32_t b = step_byte(block_max_bits(h), kFormat);
         const uint2 c = encode8(h, b, kFormat);
@@ -602,7 +611,7 @@ __global__ void __launch_bounds__(kThreads) k_swiglu_fwd(RowView gate, RowView u
       }
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) g[k] = g[k] * sigmoid(g[k]) * u[k];
+    for (int k = 0; k < 8; ++k) g[k] = g[k] * sigmoid<DT>(g[k]) * u[k];
     store_span<DT>(h.p, row * h.ld + col, left, pack<DT>(g), row_lanes());
   }
 }
@@ -630,7 +639,7 @@ __global__ void __launch_bounds__(kThreads) k_swiglu_bwd(RowView dh, Saved8 gate
     const int64_t left = live ? features - col : 0;
     float d[8], h[8];
     unpack<DT>(align_span<DT>(nd[r], dh, row * dh.ld + col, left), d);
-    swiglu_back8(d, g[r], u[r], h);
+    swiglu_back8<DT>(d, g[r], u[r], h);
     if (kSave) {
       const uint32_t b = step_byte(block_max_bits(h), sh.format);
       if (live) store_saved(sh, row, col, encode8(h, b, sh.format), b);
