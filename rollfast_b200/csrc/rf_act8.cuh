@@ -479,7 +479,9 @@ __device__ __forceinline__ void store_saved(const Saved8& s, int64_t row, int64_
 // One vector of a row held by a team of whole warps, to nearest even; columns
 // behind the last panel only take part in the shuffles.
 __device__ __forceinline__ void save_row8(const Saved8& s, int64_t row, int64_t col, int64_t n, const float (&f)[8]) {
-  const uint32_t st = step_byte(block_max_bits(f), s.format);
+  // A block behind the last feature has step 1, also where the row's
+  // normalisation has made NaNs of its zeros.
+  const uint32_t a = block_max_bits(f), st = col / kBlock8 * kBlock8 < n ? step_byte(a, s.format) : 1u;
   if (col < (n + kPanel8 - 1) / kPanel8 * kPanel8) store_saved(s, row, col, encode8(f, st, s.format), st);
 }
 

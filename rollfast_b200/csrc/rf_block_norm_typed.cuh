@@ -208,7 +208,9 @@ __device__ __forceinline__ int64_t first_step(const Common& c, int col) {
 template <int DT>
 __device__ __forceinline__ void save_raw(const Saved8& s, const Common& c, int64_t step0, int row, int col,
                                          const Raw8<DT>& raw, const float (&f)[8]) {
-  const uint32_t st = step_byte(raw_max_bits<DT>(raw), s.format);
+  // A block behind the last feature has step 1, also where the row's
+  // normalisation has made NaNs of its zeros.
+  const uint32_t a = raw_max_bits<DT>(raw), st = col / kBlock8 * kBlock8 < int(c.d) ? step_byte(a, s.format) : 1u;
   const uint2 code = encode8(f, st, s.format);
   if (col < int(s.ld)) *reinterpret_cast<uint2*>(s.codes + at(row, s.ld, col)) = code;
   if ((col & (kBlock8 - 1)) == 0 && col < (int(c.d) + kPanel8 - 1) / kPanel8 * kPanel8)
