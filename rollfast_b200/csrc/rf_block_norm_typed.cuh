@@ -204,17 +204,23 @@ __device__ __forceinline__ int64_t first_step(const Common& c, int col) {
   const int64_t scale_rows = (c.rows + 63) / 64 * 64;
   return ((int64_t(col) / kPanel8) * scale_rows) * 4 + (col % kPanel8) / kBlock8;
 }
+// Step 1 for the blocks behind the last feature of every row's last panel,
+// once for all rows: there a row that is not finite has NaNs for its zeros.
+__device__ __forceinline__ void steps_behind(const Saved8& s, const Common& c) {
+  const int first = (int(c.d) + kBlock8 - 1) / kBlock8;
+  if (!s.codes || first % 4 == 0) return;
+  uint8_t* p = s.scales + int64_t(first / 4) * s.scale_rows * 4;
+  for (int64_t row = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; row < c.rows; row += int64_t(gridDim.x) * blockDim.x)
+    for (int k = first % 4; k < 4; ++k) p[4 * row + k] = 1;
+}
 // A vector as it lies in memory (raw, f its values) into a saved row.
 template <int DT>
 __device__ __forceinline__ void save_raw(const Saved8& s, const Common& c, int64_t step0, int row, int col,
                                          const Raw8<DT>& raw, const float (&f)[8]) {
-  // A block behind the last feature has step 1, also where the row's
-  // normalisation has made NaNs of its zeros.
-  const uint32_t a = raw_max_bits<DT>(raw), st = col / kBlock8 * kBlock8 < int(c.d) ? step_byte(a, s.format) : 1u;
+  const uint32_t st = step_byte(raw_max_bits<DT>(raw), s.format);
   const uint2 code = encode8(f, st, s.format);
   if (col < int(s.ld)) *reinterpret_cast<uint2*>(s.codes + at(row, s.ld, col)) = code;
-  if ((col & (kBlock8 - 1)) == 0 && col < (int(c.d) + kPanel8 - 1) / kPanel8 * kPanel8)
-    s.scales[step0 + 4 * int64_t(row)] = uint8_t(st);
+  if ((col & (kBlock8 - 1)) == 0 && col < int(c.d)) s.scales[step0 + 4 * int64_t(row)] = uint8_t(st);
 }
 
 // An absent array, or one of this type with a stride that fits 32 bits.

@@ -78,6 +78,11 @@ __global__ void __launch_bounds__(fwd_threads(BT, kVec), 1)
       }
     }
   }
+  if (kSave) {
+    steps_behind(A.sx, c);
+    steps_behind(A.sb, c);
+    steps_behind(A.sy, c);
+  }
   __syncthreads();
   const int rows = int(c.rows);
   int64_t next = int64_t(blockIdx.x) * teams + t.id;  // up to 2^31 and a step beyond
