@@ -332,10 +332,11 @@ typedef struct rf_saved_activation {
 /* Row strides (ld*) below are in elements; a row's elements are contiguous. */
 
 /* x [rows][features] -> codes and steps, to nearest even, or stochastically:
- * a value between two grid points goes to the upper one with the probability
- * of its distance from the lower (mean = value, so gradients that are linear
- * in it stay unbiased), by 16 bits per element of the SplitMix64 sequence of
- * `seed`, in element order as in rf_apply_updates. */
+ * a value between two grid points goes to the upper one (e4m3: the larger in
+ * magnitude) with the probability of its distance from the other, rounded
+ * down to 2^-16, by 16 bits per element of the SplitMix64 sequence of `seed`,
+ * in element order as in rf_apply_updates.  The mean is the value to within
+ * 2^-16 of a step, and so are gradients that are linear in it. */
 rf_status rf_save_activation(const void* x, int64_t ldx, int32_t dtype, const rf_saved_activation* out,
                              int32_t stochastic, uint64_t seed, void* stream);
 /* The values, rounded to `dtype` (exact in float32 and bfloat16 but for
@@ -358,9 +359,12 @@ rf_status rf_swiglu_backward(const void* grad_h, int64_t ld_grad, const rf_saved
  *   layout RF_OUT_IN: out[o][i], the transpose
  * in float32, rounded once to out_dtype.  `initial` (out's shape, dtype and
  * stride) may be NULL, or out itself to accumulate in place.  X enters the
- * tensor cores exactly; float16 and float32 gradients enter as two and three
- * bfloat16 terms that add up to them exactly.  rows = 0 writes `initial` or
- * zeros.  The result does not depend on anything but the operands and their
+ * tensor cores exactly (but for subnormals); float16 and float32 gradients
+ * enter as two and three bfloat16 terms that add up to them, but for parts
+ * below 2^-133.  The workspace holds X in bfloat16, those terms (or a copy of a
+ * bfloat16 gradient whose rows start off 16-byte boundaries), and the float32
+ * parts of the tiles whose sum is split over the rows.  rows = 0 writes
+ * `initial` or zeros.  The result does not depend on anything but the operands and their
  * shapes (no atomics). */
 typedef enum rf_weight_layout { RF_IN_OUT = 0, RF_OUT_IN = 1 } rf_weight_layout;
 rf_status rf_weight_gradient_workspace_size(int64_t rows, int64_t features, int64_t n_out, const void* grad_out,

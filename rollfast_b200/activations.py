@@ -13,9 +13,12 @@ The 8-bit form cuts a row into blocks of 32 features: 32 codes (``"int8"`` or
 ``"e4m3"``) and a power-of-two step as small as the block's largest magnitude
 allows.  int8 has steps of 1/127 to 2/127 of a block's largest magnitude, e4m3
 a relative error of at most 2^-4; both take 1.03 bytes per element.  With a
-``seed``, rounding is stochastic, as in ``apply_updates``: the mean of a code
-is the value, so weight gradients, which are linear in it, stay unbiased.  A
-block with an infinity or a NaN reads as NaN throughout.
+``seed``, rounding is stochastic, as in ``apply_updates``: a value between two
+codes goes to the upper one (e4m3: the larger in magnitude) with the
+probability of its distance from the other, rounded down to 2^-16.  So the mean
+of a code is the value to within 2^-16 of a step, and weight gradients, which
+are linear in it, are unbiased to that.  A block with an infinity or a NaN
+reads as NaN throughout.
 """
 
 from __future__ import annotations
@@ -256,7 +259,11 @@ def weight_gradient(saved: SavedActivation, grad_output: torch.Tensor, *, initia
     exactly, and so does a bfloat16 gradient; a float16 or float32 gradient is
     split into two or three bfloat16 terms that add up to it (but for parts
     below 2^-133), at two or three times the work.  Equal operands give equal
-    bits.  While it runs, the call holds the activation once in bfloat16."""
+    bits.  While it runs, the call holds a workspace: the activation once in
+    bfloat16; the terms of a gradient that is not bfloat16, or one copy of a
+    bfloat16 gradient whose rows do not start on 16-byte boundaries; and, where
+    the sum over tokens is split, the float32 parts of at most 73 tiles of
+    256 x 256."""
     _require_saved(saved, "saved")
     require_cuda(grad_output, "grad_output")
     try:

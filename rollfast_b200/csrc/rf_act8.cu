@@ -10,13 +10,15 @@
 // loads in flight; others (odd widths, shifted views) through one of the
 // simple kernels below them.
 // Measured on a B200, bfloat16, int8 (a copy: 6549 GB/s): 16384 x 14336 saved
-// in 117 us (6.1 TB/s), loaded in 117, saved stochastically in 219 in either
-// format (there the generator's integer work is the bound, 28 instructions an
-// element; e4m3 took 238 while values below its normal range were looked for
-// element by element after the scaling, not two at a time before it); SwiGLU
-// 8192 x 14336 forward 165 us (5.7 TB/s), backward 172, with h saved 190.
-// 16384 x 4097, off the boundaries: saved in 76 us (4096: 41), loaded in 92
-// (40), SwiGLU forward 211 (96), backward 243 (102); there a vector takes two
+// in 115 us (6.2 TB/s), loaded in 117, saved stochastically in 219 in either
+// format (28 instructions an element, most of them the generator's; issue
+// slots are busy 71 % of the time, with 14 warps an SM at 106 registers, so
+// latency takes the rest; e4m3 took 238 while values below its normal range
+// were looked for element by element after the scaling, not two at a time
+// before it); SwiGLU 8192 x 14336 forward 164 us (5.8 TB/s), backward 170, with
+// h saved 190; float32 310, 313 and 342.
+// 16384 x 4097, off the boundaries: saved in 76 us (4096: 39), loaded in 92
+// (39), SwiGLU forward 206 (94), backward 239 (100); there a vector takes two
 // or three loads and 13 to 17 selects, and the kernels hold 16 to 24 warps an SM.
 #include "rf_act8.cuh"
 
@@ -509,7 +511,7 @@ template <int DT, int kFormat, bool kSave>
 __global__ void __launch_bounds__(kThreads) k_swiglu_bwd_typed(const void* dh, int64_t ldd, Saved8 gate, Saved8 up,
                                                                void* dgate, int64_t ldg, void* dup, int64_t ldu,
                                                                Saved8 sh, int64_t rows, int64_t features) {
-  constexpr int R = 1;  // 199 us with h saved, 205 with two rows a turn
+  constexpr int R = 1;  // two rows a turn took 3 % longer
   const int64_t col = (int64_t(blockIdx.y) * blockDim.x + threadIdx.x) * 8;
   const bool data = col + 8 <= features;  // widths here are multiples of 8
   const int64_t step = int64_t(gridDim.x) * blockDim.y * R;

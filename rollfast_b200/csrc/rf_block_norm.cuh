@@ -61,7 +61,7 @@ __device__ __forceinline__ float gate_value(float g, int act) {
 __device__ __forceinline__ float gate_slope(float a, int act) {
   return act == RF_GATE_SIGMOID ? a * (1.f - a) : act == RF_GATE_TANH ? 1.f - a * a : 1.f;
 }
-// s a(gamma) at 8 columns of a row, or a alone (times_scale false).
+// a(gamma) at 8 columns of a row, 1 without a gate.
 __device__ __forceinline__ void gate8(const Common& c, int64_t row, int64_t col, float (&f)[8]) {
   if (!c.gate.p) {
 #pragma unroll

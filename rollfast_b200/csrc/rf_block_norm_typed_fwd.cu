@@ -12,9 +12,9 @@ constexpr int kMaxFactorBytes = 4 * int(kMaxTyped) * 4;
 // registers each hold the next row's loads too.  Others: 768 without the next
 // row, since float32 takes twice the registers on its way, and so do rows off
 // the 16-byte boundaries (512 and the next row took 197 instead of 180 us for
-// 16384 x 4096 float32, 278 instead of 229 with copies; 444 instead of 293
+// 16384 x 4096 float32, 278 instead of 225 with copies; 444 instead of 290
 // for 16384 x 4097 bfloat16; bfloat16 LayerNorm with copies, the other way
-// round, 264 instead of 213 with 768).
+// round, 264 instead of 209 with 768).
 __host__ __device__ constexpr int fwd_threads(int bt, bool vec) {
   return vec && bt != RF_F32 ? kTypedThreads : kFwdThreads;
 }
@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(fwd_threads(BT, kVec), 1)
   // x' = x + normalised * mul + add;  y = normalised * pw + pb.  The columns'
   // factors lie in shared memory, one copy for the CTA's teams: in registers
   // they left none for the next row or more warps (65536 x 768 bfloat16
-  // LayerNorm 131 us, now 115; with copies 240, now 197).
+  // LayerNorm 131 us, now 115; with copies 240, now 193).
   extern __shared__ float4 factors[];  // [mul, pw, add, pb][vector][half][thread of a team]
   int col[V], n[V];
   int64_t step0[V];

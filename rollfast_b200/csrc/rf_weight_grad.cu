@@ -14,12 +14,14 @@
 // copy costs 346 / N of the product's time.  Float16 and float32 gradients
 // become two or three bfloat16 terms that add up to them.
 //
-// 8192 x 4096 x 14336, bfloat16 gradient, float32 result: 621 us with the
-// expansion, 1.55 PFLOP/s, 0.93 of the measured cuBLAS peak in a burst.
+// 8192 x 4096 x 14336, bfloat16 gradient, float32 result, with the expansion:
+// 681 to 689 us in bursts of five calls (1.40 PFLOP/s), 686 to 699 in 200 back
+// to back; added to an earlier gradient 715 to 724 and 761 to 768.  cuBLAS on
+// ready bfloat16 operands, in turn with these, 669 to 673 and 699 to 708.
 //
 // Products.  One persistent CTA pair (cluster of 2, tcgen05 cta_group::2) per
 // 256 x 256 output tile; each CTA brings 128 rows of one operand and 128
-// columns of the other, 64 tokens a step.  The sum runs over rows of both
+// columns of the other, 128 tokens a step.  The sum runs over rows of both
 // arrays, so both operands are MN-major:
 //   warps 0, 2   TMA: boxes of 128 tokens x 64 columns (128-byte swizzle) into a
 //                ring of kStages
