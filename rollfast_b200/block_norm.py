@@ -167,11 +167,11 @@ def block_norm_forward(x: torch.Tensor, branch: torch.Tensor | None = None, *, k
     Without ``branch`` (before the first block) ``y = N_pre(x)``; with
     ``pre_norm=False`` (after the last) there is no ``y``; tensors of the part
     that is left out are refused.  With ``post_norm=False`` the branch is added
-    as it is.  ``gate`` broadcasts
-    against ``x``: equal to it along the first axes, 1 along the rest, d or 1
-    along the last -- (d,), (batch, 1, d), (batch, tokens, 1), ``x``'s own
-    shape.  ``residual_scale``: a number, (d,) or one element.  x' has ``x``'s
-    dtype, ``y`` the branch's (``x``'s without one).  At most 16384 features."""
+    as it is.  ``gate`` broadcasts against ``x``: equal to it along the first
+    axes, 1 along the rest, d or 1 along the last -- (d,), (batch, 1, d),
+    (batch, tokens, 1), ``x``'s own shape.  ``residual_scale``: a number, (d,)
+    or one element.  x' has ``x``'s dtype, ``y`` the branch's (``x``'s without
+    one).  At most 16384 features."""
     require_cuda(x, "x")
     rf_dtype(x)
     shape = tuple(x.shape)

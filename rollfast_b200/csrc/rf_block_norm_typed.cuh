@@ -14,9 +14,9 @@
 // 98 us (5.5 TB/s), with the 8-bit copies 174; backward 168 us (4.8 TB/s), from
 // saved activations 186.  With copies and backward neither HBM (DRAM 44 to
 // 47 % busy) nor the issue slots (55 %) are the bound, but the latency of a
-// row's chain of sums with 16 warps an SM.  Backward beyond 4096 features a thread holds two vectors,
-// which do not fit its 128 registers (700 to 1400 bytes spilled): 8192 x 5120
-// in 194 us, 2.1 TB/s.
+// row's chain of sums with 16 warps an SM.  Backward beyond 4096 features a
+// thread holds two vectors, which do not fit its 128 registers (700 to 1400
+// bytes spilled): 8192 x 5120 in 194 us, 2.1 TB/s.
 #pragma once
 
 #include <type_traits>

@@ -70,3 +70,24 @@ def test_dropped_updates_leave_no_memory_behind(no_collector, applied):
         out, state = step(state)
         del out
         assert torch.cuda.memory_allocated() == held
+
+
+@pytest.mark.gpu
+def test_dropped_outputs_of_the_training_step_leave_no_memory_behind(no_collector):
+    import rollfast_b200 as rf
+
+    x, g = (torch.randn(300, 264, device="cuda") for _ in range(2))
+    w = torch.ones(264, device="cuda")
+
+    def step():
+        s = rf.save_activation(x)
+        o = rf.block_norm_forward(x, g, pre_weight=w, gate=w, save="int8")
+        h, sg, su = rf.swiglu_forward(x, g)
+        return (s, rf.load_activation(s), rf.weight_gradient(s, g), o, h, rf.swiglu_backward(h, sg, su, save_h="int8"),
+                rf.block_norm_backward(x, g, o.saved_x, o.saved_branch, pre_weight=w, gate=w))
+
+    step()
+    held = torch.cuda.memory_allocated()
+    for _ in range(3):
+        step()
+        assert torch.cuda.memory_allocated() == held
